@@ -50,6 +50,9 @@ typedef enum ta_b200_status_code {
  * and the pixel then takes the float16 path (result within the float16 tolerance of the
  * float16 call on (in.float() / 255).half()).  TA_B200_CONTRAST_MEAN is not available. */
 enum { TA_B200_F32 = 0, TA_B200_F16 = 1, TA_B200_U8 = 2, TA_B200_U8_F16 = 3 };
+/* The feature operators (ta_b200_group_norm, ta_b200_dropout, ta_b200_rotary) take TA_B200_F32,
+ * TA_B200_F16 and TA_B200_BF16; the image entry points refuse TA_B200_BF16. */
+enum { TA_B200_BF16 = 4 };
 enum { TA_B200_NEAREST = 0, TA_B200_BILINEAR = 1 };
 enum { TA_B200_CONTRAST_FAST = 0, TA_B200_CONTRAST_MEAN = 1 };
 
@@ -322,6 +325,111 @@ int ta_b200_sample_params(const ta_b200_sample_spec *spec, void *stream);
  * captured ta_b200_sample_params launch before replaying the graph - the values travel as
  * kernel arguments, so no host buffer has to outlive the call. */
 int ta_b200_store_words(uint64_t *dst, uint64_t a, uint64_t b, void *stream);
+
+/*
+ * ------------------------------------------------------------------ feature operators
+ * What a network does first with the images, clips and patch tokens the calls above prepare.
+ * Three feature types; sums, statistics and angles are float32 or better, results are rounded once.
+ * None has a counterpart in the reference.
+ */
+enum { TA_B200_ACT_NONE = 0, TA_B200_ACT_RELU = 1, TA_B200_ACT_SILU = 2, TA_B200_ACT_GELU = 3 };
+
+/*
+ * Group normalisation with an activation on channels-last features [n, rows, channels] (dense;
+ * rows = height x width, or frames x height x width when a clip shares its statistics):
+ *   y = act((x - mean) * rstd * weight + bias),
+ * mean and rstd = 1 / sqrt(var + eps) over the rows x (channels / groups) elements of a sample's group.
+ * GELU is the exact one (z times the normal distribution function).
+ */
+typedef struct ta_b200_group_norm_params {
+    uint32_t struct_size;       /* sizeof(ta_b200_group_norm_params) */
+    int32_t  dtype;             /* of x, y, dy, dx */
+    int32_t  param_dtype;       /* of weight, bias, dweight, dbias */
+    int32_t  activation;        /* TA_B200_ACT_* */
+    int64_t  n, rows;
+    int32_t  channels, groups;
+    float    eps;
+    int32_t  pad_;
+    const void *x;
+    const void *weight, *bias;  /* [channels], NULL = 1 / 0 */
+    void    *y;                 /* forward only; may be x */
+    float   *mean, *rstd;       /* [n, groups]: written by the forward, read by the backward call */
+    const void *dy;             /* backward only, as the fields below */
+    void    *dx;                /* NULL: not wanted; may be dy */
+    void    *dweight, *dbias;   /* [channels], NULL: not wanted; sums over all samples in a fixed order */
+    void    *scratch;           /* device memory, 16-byte aligned, no initialisation needed, reusable by the */
+    size_t   scratch_bytes;     /* next call on the same stream; ta_b200_group_norm_scratch_bytes() or more */
+} ta_b200_group_norm_params;
+
+int ta_b200_group_norm(const ta_b200_group_norm_params *p, void *stream);
+int ta_b200_group_norm_backward(const ta_b200_group_norm_params *p, void *stream);
+/* Scratch of a forward (backward == 0) or backward call with these fields, pointers included (their
+ * alignment chooses the kernel; only scratch itself need not be set).  0: none needed, or the call would be refused. */
+size_t ta_b200_group_norm_scratch_bytes(const ta_b200_group_norm_params *p, int32_t backward);
+
+/*
+ * Dropout with a mask that is computed, never stored: y = residual + keep * x / (1 - p), a dropped
+ * element contributing exactly 0 whatever x holds.  The backward pass is the same call on dy without
+ * residual.  x is dense with sizes[0..3] in memory order; the mask has the same sizes but 1 along the
+ * dimensions whose bit is set in `shared` (bit d: dimension d).  Its entry i is kept when the 32-bit number
+ *   (half(i % 8) of P(i / 8, tag)) * 65536 + (half(i % 8) of P(i / 8, tag + 1))
+ * is not below round(p * 2^32), where P(b, t) is Philox4x32-10 with key *seed and counter (b mod 2^32,
+ * b / 2^32, offset, t), tag = 0x64726F70, and half(0), half(1), ... are the low and high 16 bits of its
+ * words in order.  The result depends on these numbers only, never on the launch.
+ */
+typedef struct ta_b200_dropout_params {
+    uint32_t struct_size;       /* sizeof(ta_b200_dropout_params) */
+    int32_t  dtype;
+    int64_t  sizes[4];
+    uint32_t shared;
+    uint32_t offset;            /* separates the calls that use one seed (layers, steps) */
+    double   p;                 /* probability of dropping, 0 to 1 inclusive */
+    uint64_t seed;
+    const uint64_t *seed_ptr;   /* device; not NULL: the seed is read there when the kernel runs, `seed` is ignored */
+    const void *x;
+    const void *residual;       /* same sizes, NULL = none */
+    void    *y;                 /* may be x or residual */
+} ta_b200_dropout_params;
+
+int ta_b200_dropout(const ta_b200_dropout_params *p, void *stream);
+
+/*
+ * Rotary positions with one to three axes (e.g. time, height, width) on queries and keys.
+ * The first sections[0] + sections[1] + ... elements of a head are rotated in pairs, the rest is copied;
+ * pair j belongs to axis 0 for j < sections[0] / 2, then to axis 1, ...; (a, b) becomes
+ * (a cos t - b sin t, b cos t + a sin t), t = position on the axis * frequency.  inverse != 0 turns by -t
+ * (the backward pass).  The first `prefix` tokens of a sample (class or register tokens) are copied.
+ */
+enum { TA_B200_PAIR_INTERLEAVED = 0,   /* pair j = elements (2 j, 2 j + 1) */
+       TA_B200_PAIR_HALVES = 1 };      /* pair j = elements (j, j + half the rotated part) */
+enum { TA_B200_SPECTRUM_AXIS = 0,      /* pair m of an axis: base^(-2 m / its section) */
+       TA_B200_SPECTRUM_JOINT = 1 };   /* pair j of the head: base^(-2 j / the rotated part) */
+enum { TA_B200_POS_GRID = 0, TA_B200_POS_I64 = 1, TA_B200_POS_F32 = 2, TA_B200_POS_I32 = 3 };
+
+typedef struct ta_b200_rotary_params {
+    uint32_t struct_size;       /* sizeof(ta_b200_rotary_params) */
+    int32_t  dtype;
+    int64_t  n, tokens;         /* samples, tokens per sample (prefix included) */
+    int32_t  prefix;
+    int32_t  q_heads, k_heads;  /* 0: that tensor is absent */
+    int32_t  dim;               /* elements per head, contiguous */
+    int32_t  axes;
+    int32_t  sections[3];
+    int32_t  pairing, spectrum, inverse;
+    int32_t  position_kind;
+    double   base;
+    const void *positions;      /* I64 / F32 / I32: device; prefix tokens have entries too (not read) */
+    int64_t  position_strides[3]; /* elements per sample (0: all samples alike), token, axis */
+    int32_t  grid[3];           /* GRID: tokens after the prefix in row-major order of these sizes; the position on */
+    float    patch;             /* an axis is the index, on the last two axes plus top / patch and left / patch */
+    const float   *top, *left;  /* [n] offset of each sample's crop window in pixels, NULL = 0 */
+    const uint8_t *flip;        /* [n] 0/1: the window was mirrored, so index i of the last axis shows size - 1 - i; NULL = no */
+    const void *q, *k;
+    void    *q_out, *k_out;     /* may be q / k */
+    int64_t  q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3];   /* elements per sample, token, head */
+} ta_b200_rotary_params;
+
+int ta_b200_rotary(const ta_b200_rotary_params *p, void *stream);
 
 /*
  * Diagnostics.  ta_b200_debug_counters copies {tiles staged through shared memory,

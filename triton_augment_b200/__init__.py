@@ -13,14 +13,14 @@ from . import config, functional, transforms, utils
 from .config import disable_autotune, enable_autotune, is_autotune_enabled
 from .functional import (InterpolationMode, adjust_brightness, adjust_contrast, adjust_contrast_fast,
                          adjust_saturation, affine, apply_brightness, apply_contrast, apply_normalize,
-                         apply_saturation, center_crop, crop, fused_augment, horizontal_flip, normalize,
-                         rgb_to_grayscale, rotate)
+                         apply_saturation, center_crop, crop, dropout, fused_augment, group_norm, horizontal_flip,
+                         normalize, rgb_to_grayscale, rotary_embedding, rotate)
 from .graphs import GraphedTransform
 from .multi_gpu import ShardedAugment, ShardError, shard_bounds
-from .transforms import (TritonCenterCrop, TritonColorJitter, TritonColorJitterNormalize, TritonFusedAugment,
-                         TritonGrayscale, TritonNormalize, TritonRandomAffine, TritonRandomCrop,
-                         TritonRandomCropFlip, TritonRandomGrayscale, TritonRandomHorizontalFlip,
-                         TritonRandomRotation)
+from .transforms import (TritonCenterCrop, TritonColorJitter, TritonColorJitterNormalize, TritonDropout,
+                         TritonFusedAugment, TritonGrayscale, TritonGroupNorm, TritonNormalize, TritonRandomAffine,
+                         TritonRandomCrop, TritonRandomCropFlip, TritonRandomGrayscale, TritonRandomHorizontalFlip,
+                         TritonRandomRotation, TritonRotaryEmbedding)
 from .utils import warmup_cache
 
 __version__ = "0.3.0+b200"
@@ -34,4 +34,5 @@ __all__ = [
     "adjust_contrast_fast", "adjust_saturation", "normalize", "rgb_to_grayscale", "apply_brightness",
     "apply_contrast", "apply_saturation", "apply_normalize", "crop", "center_crop", "horizontal_flip",
     "affine", "rotate", "fused_augment", "ShardedAugment", "ShardError", "shard_bounds", "GraphedTransform",
+    "group_norm", "dropout", "rotary_embedding", "TritonGroupNorm", "TritonDropout", "TritonRotaryEmbedding",
 ]

@@ -1,0 +1,444 @@
+"""Operators on what a network makes of the augmented batch: features and patch tokens.
+
+``group_norm`` (channels-last features, with an activation), ``dropout`` (mask computed from a counter,
+never stored) and ``rotary_embedding`` (positions with one to three axes).  float32, float16 and
+bfloat16 CUDA tensors, differentiable once; each call is one call into libta_b200.so on torch's
+current stream.  No counterpart in the reference.
+
+A CUDA graph may hold forward and backward of these operators.  As with any torch operator, no graph
+of eager calls on the same leaf tensors may be alive while a backward pass is being captured (drop
+the results of warm-up calls first): autograd would make the capturing stream wait for the stream
+of the eager call.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from . import functional as _F
+
+__all__ = ["group_norm", "dropout", "rotary_embedding"]
+
+
+# ----------------------------------------------------------------------------- checks
+def _validate_feature_tensor(tensor, name: str) -> None:
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(tensor)}")
+    if tensor.dtype not in _lib.FEATURE_CODES:
+        raise TypeError(f"{name} must be float32, float16 or bfloat16, got {tensor.dtype}")
+
+
+def _on_cuda(tensor, name: str) -> None:
+    """Checked last: everything else about a call can be refused without a GPU."""
+    if not tensor.is_cuda:
+        raise ValueError(f"{name} must be on CUDA device")
+
+
+def _like(tensor, other, name: str, shape=None) -> None:
+    """``tensor`` on the device of ``other``, with ``shape``."""
+    if tensor.device != other.device:
+        raise ValueError(f"{name} must be on {other.device}, got {tensor.device}")
+    if shape is not None and tuple(tensor.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(tensor.shape)}")
+
+
+def _choice(value, table, name: str) -> int:
+    code = table.get(value) if isinstance(value, str) else None
+    if code is None:
+        raise ValueError(f"{name} must be one of {', '.join(repr(k) for k in table)}, got {value!r}")
+    return code
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+# ----------------------------------------------------------------------------- group norm
+def _group_norm_params(xm, weight, bias, groups, eps, act, samples) -> "_lib.GroupNormParams":
+    p = _lib.GroupNormParams()
+    p.struct_size = C.sizeof(_lib.GroupNormParams)
+    p.dtype = _lib.FEATURE_CODES[xm.dtype]
+    param = weight if weight is not None else bias
+    p.param_dtype = _lib.F32 if param is None else _lib.FEATURE_CODES[param.dtype]
+    p.activation = act
+    channels = xm.shape[-1]
+    p.n, p.rows = samples, (xm.numel() // (samples * channels) if samples else 0)
+    p.channels, p.groups, p.eps = channels, groups, eps
+    p.x, p.weight, p.bias = xm.data_ptr(), _address(weight), _address(bias)
+    return p
+
+
+def _group_norm_forward(x, weight, bias, groups, eps, act, samples):
+    """Features with channels last in memory, the result, and the statistics [2, samples * groups]."""
+    xm = x.movedim(-3, -1).contiguous()
+    y = torch.empty_like(xm)
+    stats = torch.empty(2, samples * groups, dtype=torch.float32, device=x.device)
+    p = _group_norm_params(xm, weight, bias, groups, eps, act, samples)
+    p.y, p.mean, p.rstd = y.data_ptr(), stats.data_ptr(), stats.data_ptr() + 4 * samples * groups
+    _lib.launch_group_norm(p, x.device)
+    return xm, y.movedim(-1, -3), stats
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act, samples):
+        xm, y, stats = _group_norm_forward(x, weight, bias, groups, eps, act, samples)
+        ctx.save_for_backward(xm, weight, bias, stats)
+        ctx.rest = (groups, eps, act, samples)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        xm, weight, bias, stats = ctx.saved_tensors
+        groups, eps, act, samples = ctx.rest
+        dym = dy.movedim(-3, -1).contiguous()
+        p = _group_norm_params(xm, weight, bias, groups, eps, act, samples)
+        p.mean, p.rstd = stats.data_ptr(), stats.data_ptr() + 4 * samples * groups
+        p.dy = dym.data_ptr()
+        dx = torch.empty_like(xm) if ctx.needs_input_grad[0] else None
+        dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
+        db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
+        p.dx, p.dweight, p.dbias = _address(dx), _address(dw), _address(db)
+        _lib.launch_group_norm(p, xm.device, backward=True)
+        return None if dx is None else dx.movedim(-1, -3), dw, db, None, None, None, None
+
+
+def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5, activation: str = "none", *,
+               same_on_frame: bool = False) -> torch.Tensor:
+    """Group normalisation and an activation in one pass: ``act((x - mean) / sqrt(var + eps) * weight + bias)``.
+
+    ``x``: features ``(C, H, W)``, ``(N, C, H, W)`` or ``(N, T, C, H, W)`` of any channel count, channels
+    last in memory (``torch.channels_last``; each frame of a clip likewise) - any other layout is
+    copied to that one first, and the result has it.  ``mean`` and ``var`` (biased) are taken over the
+    pixels and the ``C / num_groups`` channels of a group, per image, and per frame of a clip or, with
+    ``same_on_frame=True``, over all its frames.  ``weight`` and ``bias``: ``(C,)``, both in one of the three
+    types, which need not be the features'.  ``activation``: ``"none"``, ``"relu"``, ``"silu"`` or ``"gelu"`` (exact).
+
+    Statistics and arithmetic are float32, the result is rounded once.  Differentiable in ``x``, ``weight``
+    and ``bias``; sums run in a fixed order, so results and gradients repeat bit for bit.
+    """
+    _validate_feature_tensor(x, "x")
+    if x.ndim not in (3, 4, 5):
+        raise ValueError(f"Expected 3D, 4D, or 5D tensor, got {x.ndim}D tensor with shape {x.shape}")
+    channels = x.shape[-3]
+    if isinstance(num_groups, bool) or not isinstance(num_groups, int) or num_groups <= 0:
+        raise ValueError(f"num_groups must be a positive integer, got {num_groups}")
+    if channels == 0 or channels % num_groups:
+        raise ValueError(f"{channels} channels cannot be split into {num_groups} groups")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _validate_feature_tensor(t, name)
+            _like(t, x, name, (channels,))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight and bias must have one dtype, got {weight.dtype} and {bias.dtype}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    act = _choice(activation, _lib.ACTIVATIONS, "activation")
+    _on_cuda(x, "x")
+    samples = 1 if x.ndim == 3 else x.shape[0] * (x.shape[1] if x.ndim == 5 and not same_on_frame else 1)
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if _wants_grad(x, weight, bias):
+        return _GroupNorm.apply(x, weight, bias, num_groups, float(eps), act, samples)
+    return _group_norm_forward(x, weight, bias, num_groups, float(eps), act, samples)[1]
+
+
+# ----------------------------------------------------------------------------- dropout
+_MODES = {"element": 0, "channel": 1, "pixel": 2, "sample": 3}
+
+
+def _memory_order(x):
+    """``x`` dense in memory order, and whether that order has the channels last."""
+    if x.is_contiguous():
+        return x, False
+    if x.ndim in (3, 4, 5):
+        last = x.movedim(-3, -1)
+        if last.is_contiguous():
+            return last, True
+    return x.contiguous(), False
+
+
+def _mask_layout(shape, channels_last, mode, same_on_batch, same_on_frame):
+    """Four sizes of the tensor in memory order and the bit set of those the mask is shared along."""
+    if mode == 0 and not (same_on_batch or same_on_frame):
+        return (1, 1, 1, torch.Size(shape).numel()), 0
+    n = shape[0] if len(shape) >= 4 else 1
+    t = shape[1] if len(shape) == 5 else 1
+    c, plane = shape[-3], shape[-2] * shape[-1]
+    chan_bit, plane_bit = (8, 4) if channels_last else (4, 8)
+    shared = ((1 if same_on_batch else 0) | (2 if same_on_frame else 0) | (plane_bit if mode in (1, 3) else 0)
+              | (chan_bit if mode in (2, 3) else 0))
+    return ((n, t, plane, c) if channels_last else (n, t, c, plane)), shared
+
+
+def _dropout_launch(xm, residual, layout, p, seed, seed_tensor, offset):
+    y = torch.empty_like(xm)
+    a = _lib.DropoutParams()
+    a.struct_size = C.sizeof(_lib.DropoutParams)
+    a.dtype = _lib.FEATURE_CODES[xm.dtype]
+    a.sizes[:], a.shared = layout
+    a.offset, a.p, a.seed = offset, p, seed
+    a.seed_ptr = _address(seed_tensor)
+    a.x, a.residual, a.y = xm.data_ptr(), _address(residual), y.data_ptr()
+    _lib.launch_dropout(a, xm.device)
+    return y
+
+
+def _dropout_forward(x, residual, p, seed, seed_tensor, offset, mode, same_on_batch, same_on_frame):
+    xm, last = _memory_order(x)
+    layout = _mask_layout(x.shape, last, mode, same_on_batch, same_on_frame)
+    if residual is not None:
+        residual = (residual.movedim(-3, -1) if last else residual).contiguous()
+    y = _dropout_launch(xm, residual, layout, p, seed, seed_tensor, offset)
+    return (y.movedim(-1, -3) if last else y), last, layout
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, seed_tensor, offset, mode, same_on_batch, same_on_frame):
+        y, last, layout = _dropout_forward(x, residual, p, seed, seed_tensor, offset, mode, same_on_batch, same_on_frame)
+        ctx.save_for_backward(seed_tensor)
+        ctx.rest = (last, layout, p, seed, offset)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (seed_tensor,) = ctx.saved_tensors
+        last, layout, p, seed, offset = ctx.rest
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = _dropout_launch((dy.movedim(-3, -1) if last else dy).contiguous(), None, layout, p, seed, seed_tensor, offset)
+            dx = dx.movedim(-1, -3) if last else dx
+        return (dx, dy if ctx.needs_input_grad[1] else None) + (None,) * 7
+
+
+def dropout(x, p: float = 0.5, seed=None, *, offset: int = 0, mode: str = "element", same_on_batch: bool = False,
+            same_on_frame: bool = False, residual=None) -> torch.Tensor:
+    """``residual + keep * x / (1 - p)`` with a mask that is a function of ``(seed, offset, position)`` and is
+    computed where it is needed: no mask is stored, and the backward pass computes it again.
+
+    ``seed``: an integer (taken modulo 2^64), a one-element int64 tensor on ``x``'s device (read when the
+    kernel runs, so a captured graph can be replayed with another seed; do not overwrite it between a
+    forward pass and its backward pass), or None: one draw from torch's generator for that device, so
+    ``torch.manual_seed`` repeats it and replays of a captured graph differ.  ``offset`` (0 to 2^32 - 1)
+    separates calls that share a seed, such as the layers of a network.
+
+    ``mode``: what is dropped together - ``"element"`` (``x`` of any shape), or, for ``(C, H, W)``, ``(N, C, H, W)``
+    and ``(N, T, C, H, W)`` features, ``"channel"`` (whole planes), ``"pixel"`` (all channels of a pixel) or
+    ``"sample"`` (whole images; with ``residual``: stochastic depth).  ``same_on_batch`` / ``same_on_frame``: one
+    mask for all samples / for all frames of a clip, as in the transform classes (no meaning for a
+    single image; same_on_frame none for images).
+
+    A dropped element contributes exactly 0, whatever it held; ``p = 1`` drops everything.  Mask entries are
+    numbered in memory order (row-major, or channels last where ``x`` has that layout; other layouts are
+    copied to row-major), so the same values in another layout get another mask.  An element is kept
+    when its 32-bit number is not below ``round(p * 2^32)``.  The result has ``x``'s layout and is rounded
+    once.  Differentiable in ``x`` and ``residual``.
+    """
+    _validate_feature_tensor(x, "x")
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p ({p}) must be in [0, 1]")
+    code = _choice(mode, _MODES, "mode")
+    if x.ndim not in (3, 4, 5) and (code or same_on_batch or same_on_frame):
+        raise ValueError(f"mode={mode!r} and same_on_* need a 3D, 4D, or 5D tensor, got {x.ndim}D tensor with shape {x.shape}")
+    if isinstance(offset, bool) or not isinstance(offset, int) or not 0 <= offset < 2 ** 32:
+        raise ValueError(f"offset must be an integer in [0, 2^32), got {offset}")
+    if residual is not None:
+        _validate_feature_tensor(residual, "residual")
+        _like(residual, x, "residual", x.shape)
+        if residual.dtype != x.dtype:
+            raise TypeError(f"residual must be {x.dtype} like x, got {residual.dtype}")
+    number, tensor = 0, None
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise TypeError(f"a seed tensor must hold one int64, got {seed.dtype} of shape {tuple(seed.shape)}")
+        _like(seed, x, "seed")
+        tensor = seed
+    elif isinstance(seed, int) and not isinstance(seed, bool):
+        number = seed & (2 ** 64 - 1)
+    elif seed is not None:
+        raise TypeError(f"seed must be an integer, an int64 tensor or None, got {type(seed)}")
+    _on_cuda(x, "x")
+    if seed is None:
+        tensor = torch.randint(-2 ** 63, 2 ** 63 - 1, (1,), dtype=torch.int64, device=x.device)
+    same_on_batch, same_on_frame = bool(same_on_batch) and x.ndim >= 4, bool(same_on_frame) and x.ndim == 5
+    args = (p, number, tensor, offset, code, same_on_batch, same_on_frame)
+    if _wants_grad(x, residual):
+        return _Dropout.apply(x, residual, *args)
+    return _dropout_forward(x, residual, *args)[0]
+
+
+# ----------------------------------------------------------------------------- rotary positions
+class _Rotary:
+    """The part of a call that forward and backward share."""
+    __slots__ = ("sections", "base", "pairing", "spectrum", "prefix", "grid", "patch")
+
+
+def _inner_dense(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _rotary_launch(spec, q, k, positions, top, left, flip, inverse):
+    """One launch on ``q`` and ``k`` (either may be None); the results have their layouts."""
+    first = q if q is not None else k
+    a = _lib.RotaryParams()
+    a.struct_size = C.sizeof(_lib.RotaryParams)
+    a.dtype = _lib.FEATURE_CODES[first.dtype]
+    a.n, a.tokens, _, a.dim = first.shape
+    a.prefix, a.axes = spec.prefix, len(spec.sections)
+    for i, s in enumerate(spec.sections):
+        a.sections[i] = s
+    a.pairing, a.spectrum, a.inverse, a.base = spec.pairing, spec.spectrum, int(inverse), spec.base
+    if positions is not None:
+        a.position_kind, a.positions = _lib.POSITION_CODES[positions.dtype], positions.data_ptr()
+        st = positions.stride()
+        a.position_strides[:] = st if positions.ndim == 3 else (0,) + st
+    else:
+        a.position_kind = _lib.POS_GRID
+        for i, s in enumerate(spec.grid):
+            a.grid[i] = s
+        a.patch = spec.patch
+        a.top, a.left, a.flip = _address(top), _address(left), _address(flip)
+    outs = []
+    for t, name in ((q, "q"), (k, "k")):
+        if t is None:
+            outs.append(None)
+            continue
+        t = _inner_dense(t)
+        out = torch.empty_like(t)
+        if out.stride(-1) != 1:                # an expanded input: its copy is laid out by size
+            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        setattr(a, name + "_heads", t.shape[2])
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_out", out.data_ptr())
+        getattr(a, name + "_strides")[:] = t.stride()[:3]
+        getattr(a, name + "_out_strides")[:] = out.stride()[:3]
+        outs.append((t, out))
+    _lib.launch_rotary(a, first.device)
+    return tuple(None if o is None else o[1] for o in outs)
+
+
+class _RotaryEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, top, left, flip, spec):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions, top, left, flip)
+        ctx.spec = spec
+        return _rotary_launch(spec, q, k, positions, top, left, flip, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        dq = dq if ctx.needs_input_grad[0] else None
+        dk = dk if ctx.needs_input_grad[1] else None
+        if dq is not None or dk is not None:
+            dq, dk = _rotary_launch(ctx.spec, dq, dk, *ctx.saved_tensors, True)
+        return dq, dk, None, None, None, None, None
+
+
+def _per_sample(value, neutral, n, dtype, device, name):
+    """A scalar or ``(N,)`` window argument; None where it is the neutral scalar."""
+    if not isinstance(value, torch.Tensor) and value == neutral:
+        return None
+    return _F._convert_to_tensor(value, n, dtype, device, name)
+
+
+def rotary_embedding(q, k=None, *, sections, positions=None, grid=None, patch: float = 1, top=0, left=0,
+                     flip_horizontal=False, base: float = 10000.0, pairing: str = "interleaved", spectrum: str = "axis",
+                     prefix: int = 0):
+    """Rotary positions with one to three axes on queries ``(N, L, heads, D)`` and, in the same launch, keys
+    ``(N, L, key heads, D)``.  Returns the rotated ``q``, or ``(q, k)`` when keys are given.
+
+    ``sections``: for each axis (time, height, width or fewer) how many elements of a head it rotates, even
+    numbers whose sum is at most ``D`` (and 512); what is left is copied.  ``pairing="interleaved"`` turns elements
+    ``(2j, 2j + 1)``, ``"halves"`` elements ``(j, j + sum(sections) / 2)``; pairs go to the axes in order.  With
+    ``spectrum="axis"`` pair ``m`` of an axis has frequency ``base ** (-2m / its section)``, with ``"joint"`` pair ``j`` of
+    the head has ``base ** (-2j / sum(sections))``.
+
+    Positions come from one of two arguments.  ``positions``: an int64, int32 or float32 tensor ``(L, axes)`` or
+    ``(N, L, axes)`` (tokens of text and of images mixed, single tokens while generating, frame times).
+    ``grid``: the patch grid, one size per axis, tokens in row-major order; the index is the position.
+    With ``grid``, the window arguments of :func:`fused_augment` keep the patches of a crop at the places
+    they had in the whole image: ``top`` and ``left`` (pixels, numbers or ``(N,)`` tensors) move the height and
+    width axes by ``top / patch`` and ``left / patch``, where a patch is ``patch`` pixels wide, and for samples
+    selected by ``flip_horizontal`` the columns count from the other side.
+
+    The first ``prefix`` tokens of every sample (class or register tokens) are copied; ``grid`` does not
+    count them, ``positions`` has (unused) entries for them.  Angles are reduced before they are rounded, so
+    positions up to 2^24 in size lose nothing; strided views, such as slices of a fused projection or transposed
+    ``(N, heads, L, D)`` tensors, are read in place, and results have the layout ``torch.empty_like`` gives.
+    Differentiable in ``q`` and ``k``, not in positions.
+    """
+    _validate_feature_tensor(q, "q")
+    if q.ndim != 4:
+        raise ValueError(f"q must have shape (N, L, heads, D), got {tuple(q.shape)}")
+    n, length, _, dim = q.shape
+    if k is not None:
+        _validate_feature_tensor(k, "k")
+        if k.ndim != 4:
+            raise ValueError(f"k must have shape (N, L, heads, D), got {tuple(k.shape)}")
+        _like(k, q, "k", (n, length, k.shape[2], dim))
+        if k.dtype != q.dtype:
+            raise TypeError(f"k must be {q.dtype} like q, got {k.dtype}")
+    spec = _Rotary()
+    spec.sections = tuple(int(s) for s in sections)
+    axes = len(spec.sections)
+    if not 1 <= axes <= 3:
+        raise ValueError(f"sections must name one to three axes, got {axes}")
+    if any(s < 0 or s % 2 for s in spec.sections) or sum(spec.sections) > min(dim, 512):
+        raise ValueError(f"sections must be even, not negative, and add up to at most {min(dim, 512)}, got {spec.sections}")
+    spec.base = float(base)
+    if not 0.0 < spec.base < float("inf"):
+        raise ValueError(f"base must be positive, got {base}")
+    spec.pairing = _choice(pairing, _lib.PAIRINGS, "pairing")
+    spec.spectrum = _choice(spectrum, _lib.SPECTRA, "spectrum")
+    spec.prefix = int(prefix)
+    if not 0 <= spec.prefix <= length:
+        raise ValueError(f"prefix must be in [0, {length}], got {prefix}")
+    if (positions is None) == (grid is None):
+        raise ValueError("exactly one of positions and grid must be given")
+    spec.grid = spec.patch = top_t = left_t = flip_t = None
+    window = [name for name, v in (("top", top), ("left", left), ("flip_horizontal", flip_horizontal))
+              if isinstance(v, torch.Tensor) or v]
+    if positions is not None:
+        if not isinstance(positions, torch.Tensor):
+            raise TypeError(f"positions must be a torch.Tensor, got {type(positions)}")
+        if positions.dtype not in _lib.POSITION_CODES:
+            raise TypeError(f"positions must be int64, int32 or float32, got {positions.dtype}")
+        if tuple(positions.shape) not in ((length, axes), (n, length, axes)):
+            raise ValueError(f"positions must have shape ({length}, {axes}) or ({n}, {length}, {axes}), got {tuple(positions.shape)}")
+        _like(positions, q, "positions")
+        if positions.requires_grad:
+            raise ValueError("positions must not require gradients")
+        if window or patch != 1:
+            raise ValueError(f"{', '.join(window) or 'patch'} belongs to grid, not to positions")
+    else:
+        spec.grid = tuple(int(g) for g in ((grid,) if isinstance(grid, int) else grid))
+        if len(spec.grid) != axes or any(g < 0 for g in spec.grid):
+            raise ValueError(f"grid must have {axes} sizes like sections, got {grid}")
+        if torch.Size(spec.grid).numel() != length - spec.prefix:
+            raise ValueError(f"grid {spec.grid} has {torch.Size(spec.grid).numel()} patches for {length - spec.prefix} tokens")
+        spec.patch = float(patch)
+        if not 0.0 < spec.patch < float("inf"):
+            raise ValueError(f"patch must be positive, got {patch}")
+        if axes < 2 and "top" in window:
+            raise ValueError("top needs a height axis")
+        _on_cuda(q, "q")
+        top_t = _per_sample(top, 0, n, torch.float32, q.device, "top")
+        left_t = _per_sample(left, 0, n, torch.float32, q.device, "left")
+        flip_t = _per_sample(flip_horizontal, False, n, torch.bool, q.device, "flip_horizontal")
+    _on_cuda(q, "q")
+    if _wants_grad(q, k):
+        out_q, out_k = _RotaryEmbedding.apply(q, k, positions, top_t, left_t, flip_t, spec)
+    else:
+        out_q, out_k = _rotary_launch(spec, q, k, positions, top_t, left_t, flip_t, False)
+    return out_q if k is None else (out_q, out_k)

@@ -16,6 +16,13 @@ LIB_PATH = os.environ.get("TA_B200_LIB") or os.path.join(_HERE, "lib", "libta_b2
 
 ABI_VERSION = 1
 F32, F16, U8, U8_F16 = 0, 1, 2, 3       # U8 / U8_F16: bytes in (read as value / 255), float32 / float16 out
+BF16 = 4                                # feature operators only, next to F32 and F16
+FEATURE_CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+PAIRINGS = {"interleaved": 0, "halves": 1}
+SPECTRA = {"axis": 0, "joint": 1}
+POS_GRID = 0
+POSITION_CODES = {torch.int64: 1, torch.float32: 2, torch.int32: 3}
 NEAREST, BILINEAR = 0, 1
 CONTRAST_FAST, CONTRAST_MEAN = 0, 1
 ERR_TIMEOUT = -9
@@ -29,7 +36,8 @@ SYMBOLS = (
     "ta_b200_debug_crop_path", "ta_b200_debug_host_upload", "ta_b200_sample_params",
     "ta_b200_debug_tile_shape", "ta_b200_status", "ta_b200_host_release", "ta_b200_debug_wait",
     "ta_b200_fused_augment_mean", "ta_b200_fused_augment_mean_scratch_bytes", "ta_b200_mean_path",
-    "ta_b200_store_words", "ta_b200_debug_tile_height",
+    "ta_b200_store_words", "ta_b200_debug_tile_height", "ta_b200_group_norm", "ta_b200_group_norm_backward",
+    "ta_b200_group_norm_scratch_bytes", "ta_b200_dropout", "ta_b200_rotary",
 )
 
 
@@ -65,6 +73,42 @@ class SampleSpec(C.Structure):
         ("torch_compat", C.c_int32), ("draw", C.c_int8 * 13), ("pad_", C.c_int8 * 3),
         ("torch_seed", C.c_uint64), ("torch_offset", C.c_uint64), ("torch_state", C.c_void_p),
         ("first_sample", C.c_int32), ("pad2_", C.c_int32),
+    ]
+
+
+class GroupNormParams(C.Structure):
+    """ta_b200_group_norm_params of include/ta_b200.h."""
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("activation", C.c_int32),
+        ("n", C.c_int64), ("rows", C.c_int64), ("channels", C.c_int32), ("groups", C.c_int32),
+        ("eps", C.c_float), ("pad_", C.c_int32),
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("y", C.c_void_p),
+        ("mean", C.c_void_p), ("rstd", C.c_void_p), ("dy", C.c_void_p), ("dx", C.c_void_p),
+        ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t),
+    ]
+
+
+class DropoutParams(C.Structure):
+    """ta_b200_dropout_params of include/ta_b200.h."""
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("sizes", C.c_int64 * 4), ("shared", C.c_uint32),
+        ("offset", C.c_uint32), ("p", C.c_double), ("seed", C.c_uint64), ("seed_ptr", C.c_void_p),
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
+    ]
+
+
+class RotaryParams(C.Structure):
+    """ta_b200_rotary_params of include/ta_b200.h."""
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("n", C.c_int64), ("tokens", C.c_int64),
+        ("prefix", C.c_int32), ("q_heads", C.c_int32), ("k_heads", C.c_int32), ("dim", C.c_int32),
+        ("axes", C.c_int32), ("sections", C.c_int32 * 3), ("pairing", C.c_int32), ("spectrum", C.c_int32),
+        ("inverse", C.c_int32), ("position_kind", C.c_int32), ("base", C.c_double), ("positions", C.c_void_p),
+        ("position_strides", C.c_int64 * 3), ("grid", C.c_int32 * 3), ("patch", C.c_float),
+        ("top", C.c_void_p), ("left", C.c_void_p), ("flip", C.c_void_p),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+        ("q_strides", C.c_int64 * 3), ("k_strides", C.c_int64 * 3),
+        ("q_out_strides", C.c_int64 * 3), ("k_out_strides", C.c_int64 * 3),
     ]
 
 
@@ -133,6 +177,16 @@ def load():
     lib.ta_b200_host_release.restype = C.c_int
     lib.ta_b200_debug_wait.argtypes = [C.c_uint64, C.c_int32]
     lib.ta_b200_debug_wait.restype = C.c_int
+    lib.ta_b200_group_norm.argtypes = [C.POINTER(GroupNormParams), C.c_void_p]
+    lib.ta_b200_group_norm.restype = C.c_int
+    lib.ta_b200_group_norm_backward.argtypes = [C.POINTER(GroupNormParams), C.c_void_p]
+    lib.ta_b200_group_norm_backward.restype = C.c_int
+    lib.ta_b200_group_norm_scratch_bytes.argtypes = [C.POINTER(GroupNormParams), C.c_int32]
+    lib.ta_b200_group_norm_scratch_bytes.restype = C.c_size_t
+    lib.ta_b200_dropout.argtypes = [C.POINTER(DropoutParams), C.c_void_p]
+    lib.ta_b200_dropout.restype = C.c_int
+    lib.ta_b200_rotary.argtypes = [C.POINTER(RotaryParams), C.c_void_p]
+    lib.ta_b200_rotary.restype = C.c_int
     if lib.ta_b200_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libta_b200.so has ABI {lib.ta_b200_abi_version()}, this package expects {ABI_VERSION}")
     _lib = lib
@@ -316,6 +370,31 @@ def store_words(dst: torch.Tensor, a: int, b: int) -> None:
     with torch.cuda.device(dst.device):
         stream = C.c_void_p(torch.cuda.current_stream(dst.device).cuda_stream)
         check(load().ta_b200_store_words(_ptr(dst), int(a) & (2 ** 64 - 1), int(b) & (2 ** 64 - 1), stream), "ta_b200_store_words")
+
+
+def launch_group_norm(params: GroupNormParams, device: torch.device, backward: bool = False) -> None:
+    """Enqueue a group norm (or its backward pass) with the scratch it asks for."""
+    lib = load()
+    with _OnDevice(device):
+        need = int(lib.ta_b200_group_norm_scratch_bytes(C.byref(params), int(backward)))
+        if need:
+            scratch = torch.empty(need, dtype=torch.uint8, device=device)      # stream-ordered: may be released after the launch
+            params.scratch, params.scratch_bytes = scratch.data_ptr(), need
+        fn, name = ((lib.ta_b200_group_norm_backward, "ta_b200_group_norm_backward") if backward
+                    else (lib.ta_b200_group_norm, "ta_b200_group_norm"))
+        check(fn(C.byref(params), _stream(device)), name)
+
+
+def launch_dropout(params: DropoutParams, device: torch.device) -> None:
+    lib = load()
+    with _OnDevice(device):
+        check(lib.ta_b200_dropout(C.byref(params), _stream(device)), "ta_b200_dropout")
+
+
+def launch_rotary(params: RotaryParams, device: torch.device) -> None:
+    lib = load()
+    with _OnDevice(device):
+        check(lib.ta_b200_rotary(C.byref(params), _stream(device)), "ta_b200_rotary")
 
 
 def crop_path(path: int) -> None:

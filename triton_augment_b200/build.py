@@ -21,7 +21,8 @@ OBJ = os.path.join(HERE, "lib", "obj")
 LIB = os.path.join(HERE, "lib", "libta_b200.so")
 
 UNITS = (["ta_api.cu", "ta_inst_f32_crop_staged.cu", "ta_inst_f32_bilinear_mix.cu", "ta_inst_f32_mean.cu",
-          "ta_inst_f32_two_phase.cu"]
+          "ta_inst_f32_two_phase.cu", "ta_dropout.cu", "ta_rotary.cu"]
+         + [f"ta_inst_gn_{t}.cu" for t in ("f32", "f16", "bf16")]
          + [f"ta_inst_f32_short_{k}.cu" for k in ("crop_staged", "nearest", "bilinear", "bilinear_mix")]
          + [f"ta_inst_f16_short_{k}.cu" for k in ("nearest", "bilinear")]
          + [f"ta_inst_u8_{k}.cu" for k in ("crop_staged", "nearest", "bilinear", "bilinear_mix")]

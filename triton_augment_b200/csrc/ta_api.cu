@@ -500,3 +500,5 @@ extern "C" int ta_b200_gray_mean_static(const ta_b200_fused_params *p, float *me
 {
     return ta::gray_mean_static(ta::Imported(p).ptr, mean_out, (cudaStream_t)stream);
 }
+
+#include "ta_api_features.cuh"

@@ -1,6 +1,8 @@
 // Second half of ta_api.cu: the two helper kernels and the extern "C" functions.
 #pragma once
 
+#include "ta_philox.cuh"
+
 namespace ta {
 
 // ----------------------------------------------------------------------------- grayscale mean
@@ -390,22 +392,8 @@ __global__ void inverse_matrix_kernel(int n, const float *center, const float *a
 }
 
 // ----------------------------------------------------------------------------- fused parameter sampler
-// Philox4x32-10 (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", SC'11): a
-// counter-based generator, so the parameter set p of a call is a pure function of (seed, p)
-// and samples that share a parameter set simply compute it again.
-__device__ __forceinline__ uint4 philox4x32_10(uint2 key, uint4 ctr)
-{
-#pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        const uint32_t hi0 = __umulhi(0xD2511F53u, ctr.x), lo0 = 0xD2511F53u * ctr.x;
-        const uint32_t hi1 = __umulhi(0xCD9E8D57u, ctr.z), lo1 = 0xCD9E8D57u * ctr.z;
-        ctr = make_uint4(hi1 ^ ctr.y ^ key.x, lo1, hi0 ^ ctr.w ^ key.y, lo0);
-        key.x += 0x9E3779B9u;
-        key.y += 0xBB67AE85u;
-    }
-    return ctr;
-}
-
+// The generator is counter-based (ta_philox.cuh): the parameter set p of a call is a pure function of
+// (seed, p) and samples that share a parameter set simply compute it again.
 __device__ __forceinline__ float unit_float(uint32_t bits) { return (float)(bits >> 8) * (1.0f / 16777216.0f); }   // [0, 1)
 __device__ __forceinline__ float uniform_in(uint32_t bits, const float (&r)[2]) { return r[0] == r[1] ? r[0] : r[0] + unit_float(bits) * (r[1] - r[0]); }
 

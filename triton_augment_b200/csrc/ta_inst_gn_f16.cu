@@ -1,0 +1,4 @@
+#include "ta_group_norm.cuh"
+namespace ta {
+cudaError_t launch_group_norm_f16(const GnArgs &a, bool backward, cudaStream_t stream) { return gn_launch<__half>(a, backward, stream); }
+}

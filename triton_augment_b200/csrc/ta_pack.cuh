@@ -1,0 +1,82 @@
+// Vectors of V elements of a feature tensor: one memory access each, converted to and from float.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace ta {
+
+template <typename T> struct FeatElem;
+template <> struct FeatElem<float> {
+    static __device__ __forceinline__ float to_f(float v) { return v; }
+    static __device__ __forceinline__ float from_f(float v) { return v; }
+    static __device__ __forceinline__ float2 to_f2(float2 v) { return v; }
+    static __device__ __forceinline__ float2 from_f2(float a, float b) { return make_float2(a, b); }
+    using Pair = float2;
+};
+template <> struct FeatElem<__half> {
+    static __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ float2 to_f2(__half2 v) { return __half22float2(v); }
+    static __device__ __forceinline__ __half2 from_f2(float a, float b) { return __floats2half2_rn(a, b); }
+    using Pair = __half2;
+};
+template <> struct FeatElem<__nv_bfloat16> {
+    static __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ float2 to_f2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+    static __device__ __forceinline__ __nv_bfloat162 from_f2(float a, float b) { return __floats2bfloat162_rn(a, b); }
+    using Pair = __nv_bfloat162;
+};
+
+template <int BYTES> struct RawOf;
+template <> struct RawOf<2> { using type = unsigned short; };
+template <> struct RawOf<4> { using type = unsigned; };
+template <> struct RawOf<8> { using type = uint2; };
+template <> struct RawOf<16> { using type = uint4; };
+
+// V elements, V * sizeof(T) in {2, 4, 8, 16} bytes and aligned to that
+template <typename T, int V> struct Pack {
+    using Raw = typename RawOf<V * sizeof(T)>::type;
+    union { Raw raw; T v[V]; typename FeatElem<T>::Pair p[V > 1 ? V / 2 : 1]; };
+    __device__ __forceinline__ Pack() {}
+    __device__ __forceinline__ void load(const T *ptr) { raw = *reinterpret_cast<const Raw *>(ptr); }
+    // read once, by this thread only: does not stay in the L1 cache
+    __device__ __forceinline__ void load_stream(const T *ptr) { raw = __ldcs(reinterpret_cast<const Raw *>(ptr)); }
+    __device__ __forceinline__ void store(T *ptr) const { *reinterpret_cast<Raw *>(ptr) = raw; }
+    __device__ __forceinline__ void unpack(float (&f)[V]) const
+    {
+        if constexpr (V == 1) f[0] = FeatElem<T>::to_f(v[0]);
+        else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float2 t = FeatElem<T>::to_f2(p[i]);
+                f[2 * i] = t.x; f[2 * i + 1] = t.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void pack(const float (&f)[V])
+    {
+        if constexpr (V == 1) v[0] = FeatElem<T>::from_f(f[0]);
+        else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) p[i] = FeatElem<T>::from_f2(f[2 * i], f[2 * i + 1]);
+        }
+    }
+};
+
+// Feature types by their TA_B200_* code (0 float32, 1 float16, 4 bfloat16), for operands that are read a few times per thread
+__device__ __forceinline__ float load_code(const void *p, int code, long long i)
+{
+    return code == 0 ? static_cast<const float *>(p)[i]
+         : code == 1 ? __half2float(static_cast<const __half *>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+__device__ __forceinline__ void store_code(void *p, int code, long long i, float v)
+{
+    if (code == 0) static_cast<float *>(p)[i] = v;
+    else if (code == 1) static_cast<__half *>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+}  // namespace ta

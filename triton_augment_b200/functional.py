@@ -18,6 +18,7 @@ __all__ = [
     "adjust_brightness", "adjust_contrast", "adjust_contrast_fast", "adjust_saturation", "normalize",
     "apply_brightness", "apply_contrast", "apply_saturation", "apply_normalize", "rgb_to_grayscale",
     "crop", "center_crop", "horizontal_flip", "affine", "rotate", "fused_augment",
+    "group_norm", "dropout", "rotary_embedding",
 ]
 
 _DEG2RAD = 3.141592653589793 / 180.0
@@ -330,3 +331,4 @@ def _flags_from_values(angle, translate, scale, shear, bf_arg, cf_arg, sf_arg, g
 
 from ._functional_ops import *  # noqa: E402,F401,F403  (stand-alone functionals built on _run_fused)
 from ._functional_ops import apply_brightness, apply_contrast, apply_normalize, apply_saturation  # noqa: E402,F401
+from ._functional_features import (_MODES, _choice, dropout, group_norm, rotary_embedding)  # noqa: E402,F401  (features and tokens)

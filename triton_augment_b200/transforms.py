@@ -21,6 +21,7 @@ __all__ = [
     "TritonColorJitter", "TritonNormalize", "TritonColorJitterNormalize", "TritonGrayscale",
     "TritonRandomGrayscale", "TritonRandomCrop", "TritonCenterCrop", "TritonRandomHorizontalFlip",
     "TritonRandomCropFlip", "TritonRandomRotation", "TritonRandomAffine", "TritonFusedAugment",
+    "TritonGroupNorm", "TritonDropout", "TritonRotaryEmbedding",
 ]
 
 
@@ -198,3 +199,4 @@ class _BatchAware(nn.Module):
 from ._transforms_color import *      # noqa: E402,F401,F403
 from ._transforms_geometric import *  # noqa: E402,F401,F403
 from ._transforms_fused import *      # noqa: E402,F401,F403
+from ._transforms_features import *   # noqa: E402,F401,F403
