@@ -22,8 +22,8 @@ static int group_norm_args(const ta_b200_group_norm_params *p, bool backward, Gn
         return fail(TA_B200_ERR_SHAPE, "bad sizes n=%lld rows=%lld channels=%d groups=%d (channels must be a multiple of groups)",
                     (long long)p->n, (long long)p->rows, p->channels, p->groups);
     if (!(p->eps >= 0.0f)) return fail(TA_B200_ERR_SHAPE, "eps must not be negative");
-    if (p->n >= (1 << 22) || p->rows >= (1LL << 31) || (double)p->n * p->rows * p->channels >= 1.0e15)
-        return fail(TA_B200_ERR_TOO_LARGE, "at most 2^22 samples of 2^31 rows per call");
+    if (p->n >= (1 << 22) || p->rows >= (1LL << 31) || p->channels > (1 << 22) || (double)p->n * p->rows * p->channels >= 1.0e15)
+        return fail(TA_B200_ERR_TOO_LARGE, "at most 2^22 samples, 2^31 rows and 2^22 channels per call");
     const bool empty = p->n == 0 || p->rows == 0;
     if (!empty && (!p->x || (backward ? !p->dy || !p->mean || !p->rstd : !p->y || !p->mean || !p->rstd)))
         return fail(TA_B200_ERR_NULL, "x, mean, rstd and y (forward) or dy (backward) are required");
@@ -35,6 +35,7 @@ static int group_norm_args(const ta_b200_group_norm_params *p, bool backward, Gn
     a.part = (float2 *)p->scratch;
     a.n = p->n; a.rows = p->rows; a.channels = p->channels; a.groups = p->groups; a.cpg = p->channels / p->groups;
     a.param_code = p->param_dtype; a.act = p->activation; a.eps = p->eps;
+    a.wide_params = p->param_dtype == TA_B200_F32 && (((uintptr_t)p->weight | (uintptr_t)p->bias) % 16) == 0;
     return TA_B200_OK;
 }
 
@@ -117,8 +118,11 @@ static int dropout(const ta_b200_dropout_params *p, cudaStream_t stream)
     }
     const double scaled = p->p * 4294967296.0;
     const uint64_t thr = (uint64_t)nearbyint(scaled);               // p = 1: 2^32, above every number
-    a.thr_hi = (uint32_t)(thr >> 16);
+    a.drop_all = thr >> 32 != 0;
+    a.thr_hi = (uint32_t)(thr >> 16) & 0xFFFFu;
     a.thr_lo = (uint32_t)(thr & 0xFFFFu);
+    if (a.numel < (1LL << 32))
+        for (int d = 0; d < 4; ++d) a.div[d] = fast_div_of((uint32_t)a.size[d]);
     a.scale = p->p < 1.0 ? (float)(1.0 / (1.0 - p->p)) : 0.0f;
     a.sm_count = s->sm_count;
     cudaError_t e = launch_dropout(a, p->dtype, stream);

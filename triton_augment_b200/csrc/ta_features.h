@@ -13,10 +13,11 @@ struct GnArgs {
     const void *x, *weight, *bias, *dy;
     void *y, *dx, *dweight, *dbias;
     float *mean, *rstd;             // [n, groups]
-    float2 *part;                   // scratch, see group_norm_scratch_bytes()
+    float2 *part, *channel_part;    // scratch, see group_norm_scratch_bytes()
     long long n, rows;
     int channels, groups, cpg;      // cpg = channels / groups
     int param_code, act;
+    int wide_params;                // weight and bias: float32 on 16-byte boundaries
     float eps;
     int sm_count;
 };
@@ -27,6 +28,22 @@ cudaError_t launch_group_norm_f32(const GnArgs &a, bool backward, cudaStream_t s
 cudaError_t launch_group_norm_f16(const GnArgs &a, bool backward, cudaStream_t stream);
 cudaError_t launch_group_norm_bf16(const GnArgs &a, bool backward, cudaStream_t stream);
 
+// n / d for 32-bit n by a multiplication (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994)
+struct FastDiv {
+    uint32_t d, m, s1, s2;
+};
+inline FastDiv fast_div_of(uint32_t d)
+{
+    uint32_t l = 0;
+    while (l < 32 && (1ull << l) < d) ++l;
+    FastDiv f;
+    f.d = d;
+    f.m = (uint32_t)((((1ull << l) - d) << 32) / d + 1);
+    f.s1 = l < 1 ? l : 1;
+    f.s2 = l < 1 ? 0 : l - 1;
+    return f;
+}
+
 struct DropoutArgs {
     const void *x, *residual;
     void *y;
@@ -34,7 +51,9 @@ struct DropoutArgs {
     uint64_t seed;
     long long numel;
     long long size[4], mstride[4];  // merged dimensions, outermost first, padded in front with size 1
-    uint32_t offset, thr_hi, thr_lo; // keep: (16-bit number, 16-bit refinement) >= (thr_hi, thr_lo); thr_hi may be 65536
+    FastDiv div[4];                 // of size[], where numel is below 2^32
+    uint32_t offset, thr_hi, thr_lo; // keep: (16-bit number, 16-bit refinement) >= (thr_hi, thr_lo)
+    int drop_all;                   // the threshold is 2^32: above every number
     float scale;
     int sm_count;
 };

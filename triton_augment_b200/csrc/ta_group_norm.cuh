@@ -7,66 +7,245 @@
 #include "ta_features.h"
 #include "ta_pack.cuh"
 
+
 namespace ta {
 
 // ----------------------------------------------------------------------------- activations
-// FAST (results of 16 bits): the hardware's approximations, a few units of 2^-23 off, 2^-8 of half a
-// step of float16; float32 results take the library functions.
-template <bool FAST> __device__ __forceinline__ float exp_of(float x) { return FAST ? __expf(x) : expf(x); }
-template <bool FAST> __device__ __forceinline__ float sigmoid_of(float z)
+// FAST (results of 16 bits): the hardware's exponential and reciprocal, each within 2^-22, a sixteenth
+// of a float16's half step at most after three of them; float32 results take the library functions.
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float rcp_fast(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+constexpr float kLog2E = 1.4426950408889634f;
+
+// 1 / (1 + e^-z).  (One reciprocal for two values, 1 / (d0 d1) times the other factor, would spare the special
+// function unit a quarter of its work, but costs eight more instructions per pair: these kernels wait for
+// instruction issue first.)
+template <bool FAST> __device__ __forceinline__ float2 sigmoid2(float2 z)
 {
-    const float d = 1.0f + exp_of<FAST>(-z);
-    return FAST ? __fdividef(1.0f, d) : 1.0f / d;
+#ifdef GN_PAIR
+    if constexpr (FAST) {
+    const float2 e = mul2(z, both(-kLog2E));
+    const float2 d = add2(make_float2(exp2_fast(fminf(e.x, 60.0f)), exp2_fast(fminf(e.y, 60.0f))), both(1.0f));
+    const float r = rcp_fast(d.x * d.y);
+    return make_float2(r * d.y, r * d.x);
+    }
+#endif
+    if constexpr (!FAST) return make_float2(1.0f / (1.0f + expf(-z.x)), 1.0f / (1.0f + expf(-z.y)));
+    const float2 e = mul2(z, both(-kLog2E)), d = add2(make_float2(exp2_fast(e.x), exp2_fast(e.y)), both(1.0f));
+    return make_float2(rcp_fast(d.x), rcp_fast(d.y));
 }
 
-template <bool FAST, int V> __device__ __forceinline__ void activate(int act, float (&z)[V])
+// Normal distribution function, and its density through `density`.  FAST: Abramowitz and Stegun 7.1.26,
+// erf(x) = 1 - (a1 t + ... + a5 t^5) e^-x^2 with t = 1 / (1 + p x), off by 1.5e-7 at most, which shares its exponential with the density.
+template <bool FAST> __device__ __forceinline__ float normal_cdf(float z, float &density)
 {
-    if (act == kActSilu) {
+    if constexpr (!FAST) {
+        density = 0.3989422804014327f * expf(-0.5f * z * z);
+        return fmaf(0.5f, erff(z * 0.7071067811865476f), 0.5f);
+    }
+    const float x = fabsf(z) * 0.7071067811865476f, e = exp2_fast(-kLog2E * x * x), t = rcp_fast(fmaf(0.3275911f, x, 1.0f));
+    density = 0.3989422804014327f * e;
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float upper = 0.5f * poly * e;                  // 1 - cdf(|z|)
+    return z < 0.0f ? upper : 1.0f - upper;
+}
+
+template <int ACT, bool FAST, int P> __device__ __forceinline__ void activate(float2 (&z)[P])
+{
+    if constexpr (ACT == kActSilu) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = z[i] * sigmoid_of<FAST>(z[i]);
-    } else if (act == kActRelu) {
+        for (int i = 0; i < P; ++i) z[i] = mul2(z[i], sigmoid2<FAST>(z[i]));
+    } else if constexpr (ACT == kActRelu) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = z[i] < 0.0f ? 0.0f : z[i];          // a NaN stays
-    } else if (act == kActGelu) {
+        for (int i = 0; i < P; ++i) z[i] = make_float2(z[i].x < 0.0f ? 0.0f : z[i].x, z[i].y < 0.0f ? 0.0f : z[i].y);          // a NaN stays
+    } else if constexpr (ACT == kActGelu) {
+        float density;
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = z[i] * normcdff(z[i]);
+        for (int i = 0; i < P; ++i) z[i] = make_float2(z[i].x * normal_cdf<FAST>(z[i].x, density), z[i].y * normal_cdf<FAST>(z[i].y, density));
     }
 }
 
 // g = dy * act'(z), in place of dy
-template <bool FAST, int V> __device__ __forceinline__ void activate_grad(int act, const float (&z)[V], float (&g)[V])
+template <int ACT, bool FAST, int P> __device__ __forceinline__ void activate_grad(const float2 (&z)[P], float2 (&g)[P])
 {
-    if (act == kActSilu) {
+    if constexpr (ACT == kActSilu) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float s = sigmoid_of<FAST>(z[i]);
-            g[i] *= s * (1.0f + z[i] * (1.0f - s));
+        for (int i = 0; i < P; ++i) {                     // s (1 + z (1 - s)) = s + z s - z s s
+            const float2 s = sigmoid2<FAST>(z[i]), t = mul2(z[i], s);
+            g[i] = mul2(g[i], fma2(neg2(t), s, add2(s, t)));
         }
-    } else if (act == kActRelu) {
+    } else if constexpr (ACT == kActRelu) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[i] = z[i] > 0.0f ? g[i] : 0.0f;
-    } else if (act == kActGelu) {
+        for (int i = 0; i < P; ++i) g[i] = make_float2(z[i].x > 0.0f ? g[i].x : 0.0f, z[i].y > 0.0f ? g[i].y : 0.0f);
+    } else if constexpr (ACT == kActGelu) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[i] *= normcdff(z[i]) + z[i] * 0.3989422804014327f * exp_of<FAST>(-0.5f * z[i] * z[i]);
+        for (int i = 0; i < P; ++i) {
+            float dx, dy;
+            const float cx = normal_cdf<FAST>(z[i].x, dx), cy = normal_cdf<FAST>(z[i].y, dy);
+            g[i] = mul2(g[i], fma2(z[i], make_float2(dx, dy), make_float2(cx, cy)));
+        }
     }
 }
 
-// ----------------------------------------------------------------------------- shape of the streaming kernels
-// A block covers `tile` vectors of the channel axis (all of them up to kGnThreads) and a chunk of
-// rows; thread t holds channel vector t % tile and rows t / tile, + rows_per_step, ...
-constexpr int kGnThreads = 256;
-struct GnShape { int vecs, tile, tiles, rows_per_step, chunks; long long chunk_rows; };
+// f(activation as a type): the choice is made once, outside the loops over the data
+template <int N> struct ActTag { static constexpr int value = N; };
+template <typename F> __device__ __forceinline__ void with_activation(int act, F f)
+{
+    if (act == kActSilu) f(ActTag<kActSilu>());
+    else if (act == kActGelu) f(ActTag<kActGelu>());
+    else if (act == kActRelu) f(ActTag<kActRelu>());
+    else f(ActTag<kActNone>());
+}
 
-__host__ inline GnShape gn_shape(const GnArgs &a, int v)
+// V values of a parameter vector as pairs; `value` where there is no vector.  `wide`: float32 on 16-byte boundaries.
+template <int V> __device__ __forceinline__ void load_params(const void *ptr, int code, bool wide, int first, bool active, float value, float2 (&out)[(V + 1) / 2])
+{
+#pragma unroll
+    for (int i = 0; i < (V + 1) / 2; ++i) out[i] = both(value);
+    if (!ptr || !active) return;
+    if constexpr (V >= 4) if (wide) {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            const float4 q = reinterpret_cast<const float4 *>(static_cast<const float *>(ptr) + first)[i];
+            out[2 * i] = make_float2(q.x, q.y);
+            out[2 * i + 1] = make_float2(q.z, q.w);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float t = load_code(ptr, code, first + j);
+        if (j % 2) out[j / 2].y = t;
+        else out[j / 2].x = t;
+    }
+}
+
+// (x, y) of the groups of a thread's V channels as pairs; get(group).  `group` is the group of the first
+// channel, `left` how many channels of it follow.
+template <int V, typename Get> __device__ __forceinline__ void spread_groups(int group, int left, int cpg, Get get, float2 (&x)[(V + 1) / 2], float2 (&y)[(V + 1) / 2])
+{
+    float2 t = get(group);
+    if (left >= V) {
+#pragma unroll
+        for (int i = 0; i < (V + 1) / 2; ++i) { x[i] = both(t.x); y[i] = both(t.y); }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (left == 0) { t = get(++group); left = cpg; }
+        --left;
+        if (j % 2) { x[j / 2].y = t.x; y[j / 2].y = t.y; }
+        else { x[j / 2].x = t.x; y[j / 2].x = t.y; }
+    }
+}
+
+__device__ __forceinline__ float half_of_pair(float2 v, int j) { return j % 2 ? v.y : v.x; }
+
+// Values of V channels added up over neighbours of one group, `fold` at a time, into dst[]
+template <int V> __device__ __forceinline__ void store_folded(float *dst, float (&s)[V], int fold)
+{
+    if constexpr (V >= 2) if (fold >= 2) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) s[i] += s[i + 1];
+    }
+    if constexpr (V >= 4) if (fold >= 4) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) s[i] += s[i + 2];
+    }
+    if constexpr (V >= 8) if (fold >= 8) s[0] += s[4];
+    if (fold == V) { dst[0] = s[0]; return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i % fold == 0) dst[i / fold] = s[i];
+}
+
+// How a block adds up its groups: `lanes` lanes each, the same order every time.  A group's entries are
+// `width` neighbouring values in each of a number of rows.
+struct GnLanes {
+    int lanes, width, row_step, entry_step;              // a lane's next entry: row_step rows and entry_step values on
+};
+__host__ inline GnLanes gn_lanes(int groups, int threads, int width)
+{
+    GnLanes l;
+    l.lanes = 32;
+    while (l.lanes > 1 && groups * l.lanes > threads) l.lanes >>= 1;
+    l.width = width;
+    l.row_step = l.lanes / width;
+    l.entry_step = l.lanes % width;
+    return l;
+}
+__device__ __forceinline__ float lane_sum(float v, int lanes)
+{
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_down_sync(0xffffffffu, v, o);
+    return v;
+}
+// Sum of a group's entries in its lane 0 (all threads of the block call it together)
+__device__ __forceinline__ float group_sum(const GnLanes &l, const float *red, int stride, int rows, int width, int g, bool valid)
+{
+    float s = 0.0f;
+    if (valid) {
+        const int lane = threadIdx.x & (l.lanes - 1);
+        int r = lane / l.width, e = lane - r * l.width;
+        while (r < rows) {
+            if (e < width) s += red[r * stride + g * l.width + e];
+            r += l.row_step;
+            e += l.entry_step;
+            if (e >= l.width) { e -= l.width; ++r; }
+        }
+    }
+    return lane_sum(s, l.lanes);
+}
+
+// ----------------------------------------------------------------------------- work split
+// Two launches a pass: the first reduces chunks of rows, the second reads the same rows again, last ones first
+// since those are still in the L2 cache, and writes the result.  (Ranges of samples that fit the cache, one pair
+// of launches each, were slower for all that the gaps between launches cost: 16 x 128 x 224^2 float16 in
+// 64 MB ranges 162 us, in one pair 116 us.)
+//
+// A block covers a tile of channel vectors and a chunk of rows; thread t holds vector t % tile of rows
+// t / tile + i rows_per_step.  Tiles hold whole groups (groups_per_tile); a group wider than a block is
+// cut into `split` tiles.  Each block leaves one partial result per group of its tile:
+// part[((n groups + g) chunks + chunk) split + piece].
+constexpr int kGnThreads = 256;
+constexpr int kGnBlocksForward = 4, kGnBlocksBackward = 3;       // blocks per SM (64 and 80 registers a thread)
+struct GnShape {
+    int vecs, tile, tiles, rows_per_step, groups_per_tile, split, unit, chunks, fold;
+    long long chunk_rows;
+    GnLanes columns;                    // sums over a tile's columns
+    int finish_lanes;                   // lanes a group's chunks are joined by
+};
+
+__host__ __device__ inline int gn_gcd(int a, int b) { while (b) { const int t = a % b; a = b; b = t; } return a; }
+
+// vectors of the smallest run of whole vectors that is made of whole groups
+__host__ inline int gn_unit(const GnArgs &a, int v) { return a.cpg / gn_gcd(a.cpg, v); }
+
+__host__ inline GnShape gn_shape(const GnArgs &a, int v, bool backward)
 {
     GnShape s;
     s.vecs = a.channels / v;
-    s.tile = s.vecs < kGnThreads ? s.vecs : kGnThreads;
-    s.tiles = (s.vecs + s.tile - 1) / s.tile;
+    s.unit = gn_unit(a, v);
+    if (s.unit <= kGnThreads) {
+        const int units = s.vecs / s.unit, most = kGnThreads / s.unit;
+        s.tiles = (units + most - 1) / most;
+        s.tile = (units + s.tiles - 1) / s.tiles * s.unit;
+        s.tiles = (s.vecs + s.tile - 1) / s.tile;
+        s.groups_per_tile = s.tile * v / a.cpg;
+        s.split = 1;
+    } else {                                              // gn_vector() saw to it that v divides cpg
+        s.split = (s.unit + kGnThreads - 1) / kGnThreads;
+        s.tile = (s.unit + s.split - 1) / s.split;
+        s.tiles = a.groups * s.split;
+        s.groups_per_tile = 1;
+    }
     s.rows_per_step = kGnThreads / s.tile;
-    // about eight blocks per SM, at least eight steps each, at most 512 chunks per sample
-    const long long want = (8LL * a.sm_count + a.n * s.tiles - 1) / (a.n * s.tiles);
-    const long long most = (a.rows + 8LL * s.rows_per_step - 1) / (8LL * s.rows_per_step);
+    s.fold = v;
+    while (a.cpg % s.fold) s.fold /= 2;
+    s.columns = gn_lanes(s.groups_per_tile, kGnThreads, backward ? (s.split == 1 ? a.cpg : s.tile * v) : (s.split == 1 ? a.cpg : s.tile * v) / s.fold);
+    s.finish_lanes = s.columns.lanes;
+    // one wave of blocks where the samples allow it, at least four steps a thread
+    const long long want = (long long)(backward ? kGnBlocksBackward : kGnBlocksForward) * a.sm_count / (a.n * s.tiles);
+    const long long most = (a.rows + 4LL * s.rows_per_step - 1) / (4LL * s.rows_per_step);
     long long chunks = want < most ? want : most;
     chunks = chunks > 512 ? 512 : chunks < 1 ? 1 : chunks;
     s.chunk_rows = (a.rows + chunks - 1) / chunks;
@@ -74,304 +253,461 @@ __host__ inline GnShape gn_shape(const GnArgs &a, int v)
     return s;
 }
 
-// ----------------------------------------------------------------------------- streaming kernels
-// Per (sample, chunk, channel): mean and sum of squared deviations.  A thread sums differences to the
-// first value it sees, so that a mean far from zero cancels nothing; threads are joined by Chan's rule.
-template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const GnArgs a, const GnShape s)
-{
-    const int v = threadIdx.x % s.tile, r = threadIdx.x / s.tile, vec = blockIdx.y * s.tile + v;
-    const long long item = blockIdx.x, n = item / s.chunks;
-    const int chunk = (int)(item - n * s.chunks);
-    const long long row0 = chunk * s.chunk_rows, row1 = min(row0 + s.chunk_rows, a.rows);
-    float pivot[V], sum[V], sq[V];
-    int count = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) pivot[i] = sum[i] = sq[i] = 0.0f;
-    if (r < s.rows_per_step && vec < s.vecs) {
-        const T *base = (const T *)a.x + (n * a.rows) * a.channels + (long long)vec * V;
-        for (long long row = row0 + r; row < row1; row += s.rows_per_step) {
-            Pack<T, V> p;
-            p.load(base + row * a.channels);
-            float f[V];
-            p.unpack(f);
-            if (count == 0) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) pivot[i] = f[i];
-            }
-            ++count;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float d = f[i] - pivot[i];
-                sum[i] += d;
-                sq[i] = fmaf(d, d, sq[i]);
-            }
-        }
-    }
-    __shared__ float2 acc[kGnThreads * V];      // [row slot][channel of the tile]
-    const float inv = count > 0 ? 1.0f / (float)count : 0.0f;
-    if (r < s.rows_per_step) {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            acc[(r * s.tile + v) * V + i] = make_float2(pivot[i] + sum[i] * inv, fmaxf(sq[i] - sum[i] * sum[i] * inv, 0.0f));
-    }
-    __syncthreads();
-    const long long rows = row1 - row0;
-    for (int c = threadIdx.x; c < s.tile * V; c += kGnThreads) {
-        const int channel = blockIdx.y * s.tile * V + c;
-        if (channel >= a.channels) continue;
-        float mean = 0.0f, m2 = 0.0f, total = 0.0f;
-        for (int j = 0; j < s.rows_per_step; ++j) {
-            const long long have = rows > j ? (rows - j + s.rows_per_step - 1) / s.rows_per_step : 0;
-            if (have == 0) break;
-            const float2 b = acc[j * s.tile * V + c];
-            const float nb = (float)have, delta = b.x - mean, tot = total + nb;
-            mean += delta * (nb / tot);
-            m2 += b.y + delta * delta * (total * nb / tot);
-            total = tot;
-        }
-        a.part[item * a.channels + channel] = make_float2(mean, m2);
-    }
-}
-
-__device__ __forceinline__ float warp_sum(float v)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
-// One warp per (sample, group): the partial means and deviations of its channels and chunks become mean and rstd.
-static __global__ void gn_stats_finish_kernel(const GnArgs a, const int chunks, const long long chunk_rows)
-{
-    const long long id = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-    if (id >= a.n * a.groups) return;
-    const int lane = threadIdx.x % 32;
-    const long long n = id / a.groups;
-    const int first = (int)(id - n * a.groups) * a.cpg;
-    const long long entries = (long long)chunks * a.cpg;
-    const float total = (float)a.rows * (float)a.cpg;
-    float s = 0.0f;
-    for (long long e = lane; e < entries; e += 32) {
-        const long long chunk = e / a.cpg;
-        const float rows = (float)min(chunk_rows, a.rows - chunk * chunk_rows);
-        s = fmaf(rows, a.part[(n * chunks + chunk) * a.channels + first + (e - chunk * a.cpg)].x, s);
-    }
-    // the mean in two steps: the second, around the first estimate, removes its rounding
-    float mean = warp_sum(s) / total;
-    s = 0.0f;
-    for (long long e = lane; e < entries; e += 32) {
-        const long long chunk = e / a.cpg;
-        const float rows = (float)min(chunk_rows, a.rows - chunk * chunk_rows);
-        s = fmaf(rows, a.part[(n * chunks + chunk) * a.channels + first + (e - chunk * a.cpg)].x - mean, s);
-    }
-    mean += warp_sum(s) / total;
-    s = 0.0f;
-    for (long long e = lane; e < entries; e += 32) {
-        const long long chunk = e / a.cpg;
-        const float rows = (float)min(chunk_rows, a.rows - chunk * chunk_rows);
-        const float2 p = a.part[(n * chunks + chunk) * a.channels + first + (e - chunk * a.cpg)];
-        const float d = p.x - mean;
-        s += p.y + rows * d * d;
-    }
-    const float var = warp_sum(s) / total;
-    if (lane == 0) {
-        a.mean[id] = mean;
-        a.rstd[id] = rsqrtf(var + a.eps);
-    }
-}
-
-// Per-thread constants of V channels of one sample
-template <int V> struct GnChannels {
-    float mean[V], scale[V], bias[V];       // z = (x - mean) * scale + bias
-    __device__ __forceinline__ void load(const GnArgs &a, long long n, int c0)
+// Where a thread works
+struct GnPlace {
+    int v, r, vec, vec_end, group0, piece, chunk, rows;
+    unsigned n, item;
+    long long row0;
+    bool active;
+    __device__ __forceinline__ GnPlace(const GnArgs &a, const GnShape &s, unsigned block)
     {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = c0 + i;
-            const long long g = n * a.groups + c / a.cpg;
-            mean[i] = a.mean[g];
-            scale[i] = a.rstd[g] * (a.weight ? load_code(a.weight, a.param_code, c) : 1.0f);
-            bias[i] = a.bias ? load_code(a.bias, a.param_code, c) : 0.0f;
-        }
+        r = threadIdx.x / s.tile;
+        v = threadIdx.x - r * s.tile;
+        const int tile = blockIdx.y;
+        group0 = s.split == 1 ? tile * s.groups_per_tile : tile / s.split;
+        piece = s.split == 1 ? 0 : tile - group0 * s.split;
+        const int start = s.split == 1 ? tile * s.tile : group0 * s.unit + piece * s.tile;
+        vec_end = s.split == 1 ? s.vecs : (group0 + 1) * s.unit;
+        vec = start + v;
+        n = block / (unsigned)s.chunks;
+        chunk = (int)(block - n * s.chunks);
+        item = block;
+        row0 = chunk * s.chunk_rows;
+        rows = (int)min(s.chunk_rows, a.rows - row0);
+        active = r < s.rows_per_step && vec < vec_end;
     }
+    // vectors of the tile that exist
+    __device__ __forceinline__ int width(const GnShape &s) const { return min(s.tile, vec_end - (vec - v)); }
+    __device__ __forceinline__ int groups(const GnArgs &a, const GnShape &s) const { return min(s.groups_per_tile, a.groups - group0); }
+    __device__ __forceinline__ int count(const GnShape &s) const { return active && rows > r ? (rows - r + s.rows_per_step - 1) / s.rows_per_step : 0; }
 };
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(const GnArgs a, const GnShape s)
+// The second launch of a pass may start while the first one ends (programmatic dependent launch): what
+// does not depend on the first is fetched before gn_wait_first().
+__device__ __forceinline__ void gn_allow_second() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void gn_wait_first() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+constexpr int kGnUnroll = 4;            // rows a thread has in flight
+
+// ----------------------------------------------------------------------------- forward
+// Sums of differences to a thread's pivot (its first value, negated in pv) and of their squares, per channel
+template <int P, typename Vec> __device__ __forceinline__ void add_moments(const Vec &p, const float2 (&pv)[P], float2 (&sm)[P], float2 (&s2)[P])
 {
-    const int v = threadIdx.x % s.tile, r = threadIdx.x / s.tile, vec = blockIdx.y * s.tile + v;
-    if (r >= s.rows_per_step || vec >= s.vecs) return;
-    const long long item = blockIdx.x, n = item / s.chunks;
-    const long long row0 = (item - n * s.chunks) * s.chunk_rows, row1 = min(row0 + s.chunk_rows, a.rows);
-    GnChannels<V> ch;
-    ch.load(a, n, vec * V);
-    const long long base = n * a.rows * a.channels + (long long)vec * V;
-    for (long long row = row0 + r; row < row1; row += s.rows_per_step) {
-        Pack<T, V> p;
-        p.load((const T *)a.x + base + row * a.channels);
-        float f[V];
-        p.unpack(f);
+    float2 f[P];
+    p.unpack(f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = fmaf(f[i] - ch.mean[i], ch.scale[i], ch.bias[i]);
-        activate<sizeof(T) == 2, V>(a.act, f);
-        p.pack(f);
-        p.store((T *)a.y + base + row * a.channels);
+    for (int j = 0; j < P; ++j) {
+        const float2 d = add2(f[j], pv[j]);
+        sm[j] = add2(sm[j], d);
+        s2[j] = fma2(d, d, s2[j]);
+    }
+}
+// Per channel, the squared deviations of the thread's values from its group's mean: those from the
+// thread's mean, max(s2 - sm^2 / count, 0), and count times the square of the distance of the two means
+template <int V> __device__ __forceinline__ void deviations(int group, int left, int cpg, int count, const float2 (&pv)[(V + 1) / 2],
+                                                            const float2 (&sm)[(V + 1) / 2], const float2 (&s2)[(V + 1) / 2], const float *means, float (&out)[V])
+{
+    constexpr int P = (V + 1) / 2;
+    float2 m[P], unused[P];
+    spread_groups<V>(group, left, cpg, [&](int g) { return make_float2(means[g], 0.0f); }, m, unused);
+    const float n = (float)count, inv = count > 0 ? 1.0f / n : 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float s = half_of_pair(sm[j / 2], j), q = half_of_pair(s2[j / 2], j);
+        const float own = fmaf(-s * inv, s, q), d = fmaf(s, inv, -half_of_pair(pv[j / 2], j)) - half_of_pair(m[j / 2], j);
+        out[j] = fmaf(n * d, d, own < 0.0f ? 0.0f : own);          // (a NaN stays)
     }
 }
 
-// Per (sample, chunk, channel): sums of g * xhat and of g.
+// Per (sample, group, chunk): mean and sum of squared deviations from it.  A thread sums differences to the
+// first value it sees, so that a mean far from zero cancels nothing; the block adds up its means first and
+// then the deviations from the result, and so do the chunks.
 template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads) gn_grad_sums_kernel(const GnArgs a, const GnShape s)
+__global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_stats_kernel(const GnArgs a, const GnShape s)
 {
-    const int v = threadIdx.x % s.tile, r = threadIdx.x / s.tile, vec = blockIdx.y * s.tile + v;
-    const long long item = blockIdx.x, n = item / s.chunks;
-    const long long row0 = (item - n * s.chunks) * s.chunk_rows, row1 = min(row0 + s.chunk_rows, a.rows);
-    float sum_gx[V], sum_g[V];
+    gn_allow_second();
+    const GnPlace at(a, s, blockIdx.x);
+    const int count = at.count(s);
+    constexpr int P = Pack<T, V>::P;
+    float2 pv[P], sm[P], s2[P];
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum_gx[i] = sum_g[i] = 0.0f;
-    if (r < s.rows_per_step && vec < s.vecs) {
-        GnChannels<V> ch;
-        ch.load(a, n, vec * V);
-        float rstd[V];
+    for (int j = 0; j < P; ++j) pv[j] = sm[j] = s2[j] = both(0.0f);
+    if (count > 0) {
+        const T *ptr = (const T *)a.x + (at.n * a.rows + at.row0 + at.r) * a.channels + at.vec * V;
+        const long long step = (long long)s.rows_per_step * a.channels;
+        Pack<T, V> p[kGnUnroll];
+        p[0].load(ptr);
+        p[0].unpack(pv);
 #pragma unroll
-        for (int i = 0; i < V; ++i) rstd[i] = a.rstd[n * a.groups + (vec * V + i) / a.cpg];
-        const long long base = n * a.rows * a.channels + (long long)vec * V;
-        for (long long row = row0 + r; row < row1; row += s.rows_per_step) {
-            Pack<T, V> px, pd;
-            px.load((const T *)a.x + base + row * a.channels);
-            pd.load((const T *)a.dy + base + row * a.channels);
-            float x[V], z[V], g[V];
-            px.unpack(x);
-            pd.unpack(g);
+        for (int j = 0; j < P; ++j) pv[j] = neg2(pv[j]);
+        int i = 0;
+        for (; i + kGnUnroll <= count; i += kGnUnroll, ptr += kGnUnroll * step) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) { x[i] -= ch.mean[i]; z[i] = fmaf(x[i], ch.scale[i], ch.bias[i]); }
-            activate_grad<sizeof(T) == 2, V>(a.act, z, g);
+            for (int u = 0; u < kGnUnroll; ++u) p[u].load(ptr + u * step);
 #pragma unroll
-            for (int i = 0; i < V; ++i) { sum_g[i] += g[i]; sum_gx[i] = fmaf(g[i], x[i] * rstd[i], sum_gx[i]); }
+            for (int u = 0; u < kGnUnroll; ++u) add_moments<P>(p[u], pv, sm, s2);
+        }
+        for (; i < count; ++i, ptr += step) {
+            p[0].load(ptr);
+            add_moments<P>(p[0], pv, sm, s2);
         }
     }
-    __shared__ float2 acc[kGnThreads * V];
-    if (r < s.rows_per_step) {
+    __shared__ float red[kGnThreads * V], block_mean[kGnThreads * V];       // [row slot][folded channel], [group]
+    const int per_vec = V / s.fold, stride = s.tile * per_vec, groups = at.groups(a, s);
+    const int width = s.split == 1 ? s.columns.width : at.width(s) * per_vec;
+    float *slot = red + at.r * stride + at.v * per_vec;
+    const bool holds = at.r < s.rows_per_step;
+    float t[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[(r * s.tile + v) * V + i] = make_float2(sum_gx[i], sum_g[i]);
+    for (int j = 0; j < V; ++j) t[j] = fmaf((float)-count, half_of_pair(pv[j / 2], j), half_of_pair(sm[j / 2], j));        // the plain sum
+    if (holds) store_folded<V>(slot, t, s.fold);
+    __syncthreads();
+    const float inv = 1.0f / ((float)at.rows * (float)(width * s.fold));
+    const int per_pass = kGnThreads / s.columns.lanes, lane = threadIdx.x & (s.columns.lanes - 1), mine = threadIdx.x / s.columns.lanes;
+    for (int base = 0; base < groups; base += per_pass) {
+        const int g = base + mine;
+        const float m = group_sum(s.columns, red, stride, s.rows_per_step, width, g, g < groups) * inv;
+        if (g < groups && lane == 0) block_mean[g] = m;
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < s.tile * V; c += kGnThreads) {
-        const int channel = blockIdx.y * s.tile * V + c;
-        if (channel >= a.channels) continue;
-        float2 t = make_float2(0.0f, 0.0f);
-        for (int j = 0; j < s.rows_per_step; ++j) { t.x += acc[j * s.tile * V + c].x; t.y += acc[j * s.tile * V + c].y; }
-        a.part[item * a.channels + channel] = t;
+    // deviations from the block's mean: those from the thread's own mean, and that mean's
+    deviations<V>(at.active ? (at.vec * V) / a.cpg - at.group0 : 0, at.active ? a.cpg - (at.vec * V) % a.cpg : V, a.cpg, count, pv, sm, s2, block_mean, t);
+    if (holds) store_folded<V>(slot, t, s.fold);
+    __syncthreads();
+    for (int base = 0; base < groups; base += per_pass) {
+        const int g = base + mine;
+        const float q = group_sum(s.columns, red, stride, s.rows_per_step, width, g, g < groups);
+        if (g < groups && lane == 0)
+            a.part[(((long long)at.n * a.groups + at.group0 + g) * s.chunks + at.chunk) * s.split + at.piece] = make_float2(block_mean[g], q);
     }
 }
 
-// Scratch of the backward pass: [n, chunks, C] partial sums, then [n, C] their sums over chunks, then
-// [n, G] means of (u * xhat, u) over the group.
-__device__ __forceinline__ float2 *gn_channel_sums(const GnArgs &a, int chunks) { return a.part + a.n * chunks * a.channels; }
-__device__ __forceinline__ float2 *gn_group_means(const GnArgs &a, int chunks) { return a.part + a.n * (chunks + 1) * a.channels; }
-
-// One warp per (sample, group)
-static __global__ void gn_grad_finish_kernel(const GnArgs a, const int chunks)
+// Mean and rstd of the tile's groups from their chunks, into stat[]
+__device__ __forceinline__ void gn_finish_stats(const GnArgs &a, const GnShape &s, const GnPlace &at, int v, float2 *stat)
 {
-    const long long id = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-    if (id >= a.n * a.groups) return;
-    const int lane = threadIdx.x % 32;
-    const long long n = id / a.groups;
-    const int first = (int)(id - n * a.groups) * a.cpg;
-    float2 *sums = gn_channel_sums(a, chunks);
-    float s_ux = 0.0f, s_u = 0.0f;
-    for (int i = 0; i < a.cpg; ++i) {
-        const int c = first + i;
-        float gx = 0.0f, g = 0.0f;
-        for (int chunk = lane; chunk < chunks; chunk += 32) {
-            const float2 p = a.part[(n * chunks + chunk) * a.channels + c];
-            gx += p.x; g += p.y;
-        }
-        gx = warp_sum(gx); g = warp_sum(g);
-        if (lane == 0) sums[n * a.channels + c] = make_float2(gx, g);
-        const float w = a.weight ? load_code(a.weight, a.param_code, c) : 1.0f;
-        s_ux = fmaf(w, gx, s_ux); s_u = fmaf(w, g, s_u);
-    }
+    const int groups = at.groups(a, s), lanes = s.finish_lanes, lane = threadIdx.x & (lanes - 1), entries = s.chunks * s.split;
     const float inv = 1.0f / ((float)a.rows * (float)a.cpg);
-    if (lane == 0) gn_group_means(a, chunks)[id] = make_float2(s_ux * inv, s_u * inv);
+    const auto values = [&](int e) {
+        if (s.split == 1) return (float)min(s.chunk_rows, a.rows - e * s.chunk_rows) * (float)a.cpg;
+        const int chunk = e / s.split;
+        return (float)min(s.chunk_rows, a.rows - chunk * s.chunk_rows) * (float)(min(s.tile, s.unit - (e - chunk * s.split) * s.tile) * v);
+    };
+    for (int base = 0; base < groups; base += kGnThreads / lanes) {
+        const int g = base + threadIdx.x / lanes;
+        const bool valid = g < groups;
+        const long long id = (long long)at.n * a.groups + at.group0 + g;
+        const float2 *part = a.part + id * entries;
+        // the lane's first eight entries stay in registers for the second sum
+        float2 p[8];
+        float n[8], m = 0.0f, q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = lane + i * lanes;
+            const bool have = valid && e < entries;
+            p[i] = have ? __ldcg(part + e) : make_float2(0.0f, 0.0f);
+            n[i] = have ? values(e) : 0.0f;
+            m = fmaf(n[i], p[i].x, m);
+        }
+        if (valid)
+            for (int e = lane + 8 * lanes; e < entries; e += lanes) m = fmaf(values(e), __ldcg(part + e).x, m);
+        m = __shfl_sync(0xffffffffu, lane_sum(m, lanes) * inv, 0, lanes);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (n[i] > 0.0f) q += fmaf(n[i] * (p[i].x - m), p[i].x - m, p[i].y);
+        if (valid)
+            for (int e = lane + 8 * lanes; e < entries; e += lanes) {
+                const float2 t = __ldcg(part + e);
+                q += fmaf(values(e) * (t.x - m), t.x - m, t.y);
+            }
+        q = lane_sum(q, lanes);
+        if (valid && lane == 0) {
+            const float rstd = rsqrtf(q * inv + a.eps);
+            stat[g] = make_float2(m, rstd);
+            if (at.chunk == 0 && at.piece == 0) { a.mean[id] = m; a.rstd[id] = rstd; }
+        }
+    }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads) gn_grad_input_kernel(const GnArgs a, const GnShape s)
+__global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_apply_kernel(const GnArgs a, const GnShape s)
 {
-    const int v = threadIdx.x % s.tile, r = threadIdx.x / s.tile, vec = blockIdx.y * s.tile + v;
-    if (r >= s.rows_per_step || vec >= s.vecs) return;
-    const long long item = blockIdx.x, n = item / s.chunks;
-    const long long row0 = (item - n * s.chunks) * s.chunk_rows, row1 = min(row0 + s.chunk_rows, a.rows);
-    GnChannels<V> ch;
-    ch.load(a, n, vec * V);
-    float rstd[V], m_ux[V], m_u[V];
+    extern __shared__ float2 stat[];                      // [groups_per_tile] (mean, rstd)
+    const GnPlace at(a, s, gridDim.x - 1 - blockIdx.x);        // what was read last comes first: it is in L2
+    const int count = at.count(s), c0 = at.vec * V;
+    const long long first = (at.n * a.rows + at.row0 + at.r) * a.channels + c0, step = (long long)s.rows_per_step * a.channels;
+    const T *src = (const T *)a.x + first;
+    T *dst = (T *)a.y + first;
+    constexpr int P = Pack<T, V>::P;
+    float2 mean[P], scale[P], bias[P], rstd[P];
+    load_params<V>(a.weight, a.param_code, a.wide_params, c0, at.active, 1.0f, scale);
+    load_params<V>(a.bias, a.param_code, a.wide_params, c0, at.active, 0.0f, bias);
+    const int group = at.active ? c0 / a.cpg : at.group0, left = at.active ? (group + 1) * a.cpg - c0 : V;
+    gn_wait_first();
+    gn_finish_stats(a, s, at, V, stat);
+    __syncthreads();
+    spread_groups<V>(group - at.group0, left, a.cpg, [&](int g) { return make_float2(-stat[g].x, stat[g].y); }, mean, rstd);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const long long g = n * a.groups + (vec * V + i) / a.cpg;
-        rstd[i] = a.rstd[g];
-        const float2 m = gn_group_means(a, s.chunks)[g];
-        m_ux[i] = m.x; m_u[i] = m.y;
+    for (int j = 0; j < P; ++j) scale[j] = mul2(scale[j], rstd[j]);
+    with_activation(a.act, [&](auto act) {
+        const auto apply = [&](Pack<T, V> &p, T *out) {
+            float2 f[P];
+            p.unpack(f);
+#pragma unroll
+            for (int j = 0; j < P; ++j) f[j] = fma2(add2(f[j], mean[j]), scale[j], bias[j]);
+            activate<decltype(act)::value, sizeof(T) == 2, P>(f);
+            p.pack(f);
+            p.store(out);
+        };
+        Pack<T, V> p[kGnUnroll];
+        int i = 0;
+        for (; i + kGnUnroll <= count; i += kGnUnroll, src += kGnUnroll * step, dst += kGnUnroll * step) {
+#pragma unroll
+            for (int u = 0; u < kGnUnroll; ++u) p[u].load_stream(src + u * step);
+#pragma unroll
+            for (int u = 0; u < kGnUnroll; ++u) apply(p[u], dst + u * step);
+        }
+        for (; i < count; ++i, src += step, dst += step) {
+            p[0].load_stream(src);
+            apply(p[0], dst);
+        }
+    });
+}
+
+// ----------------------------------------------------------------------------- backward
+// Scratch: [n, groups, chunks, split] sums of (u xhat, u), then [n, chunks, C] sums of (g xhat, g).
+__host__ __device__ inline float2 *gn_channel_part(const GnArgs &a, const GnShape &s) { return a.part + a.n * a.groups * s.chunks * s.split; }
+
+// acc[rows][stride]: every column's rows into its first one, by all threads: part p adds rows p, p + parts, ...
+// and then the parts are added.  Ends with the block synchronised.
+__device__ __forceinline__ void sum_columns(float2 *acc, int stride, int columns, int rows, int threads)
+{
+    int parts = threads / columns;
+    parts = parts < 1 ? 1 : parts > rows ? rows : parts;
+    for (int i = threadIdx.x; i < columns * parts; i += threads) {
+        const int part = i / columns, c = i - part * columns;
+        float2 t = acc[part * stride + c];
+#pragma unroll 4
+        for (int k = part + parts; k < rows; k += parts) { const float2 e = acc[k * stride + c]; t = add2(t, e); }
+        acc[part * stride + c] = t;
     }
-    const long long base = n * a.rows * a.channels + (long long)vec * V;
-    for (long long row = row0 + r; row < row1; row += s.rows_per_step) {
-        Pack<T, V> px, pd;
-        px.load((const T *)a.x + base + row * a.channels);
-        pd.load((const T *)a.dy + base + row * a.channels);
-        float x[V], z[V], g[V];
-        px.unpack(x);
-        pd.unpack(g);
-#pragma unroll
-        for (int i = 0; i < V; ++i) { x[i] -= ch.mean[i]; z[i] = fmaf(x[i], ch.scale[i], ch.bias[i]); }
-        activate_grad<sizeof(T) == 2, V>(a.act, z, g);
-#pragma unroll
-        for (int i = 0; i < V; ++i) g[i] = fmaf(g[i], ch.scale[i], -rstd[i] * fmaf(x[i] * rstd[i], m_ux[i], m_u[i]));
-        px.pack(g);
-        px.store((T *)a.dx + base + row * a.channels);
+    __syncthreads();
+    if (parts > 1) {
+        for (int c = threadIdx.x; c < columns; c += threads) {
+            float2 t = acc[c];
+            for (int k = 1; k < parts; ++k) t = add2(t, acc[k * stride + c]);
+            acc[c] = t;
+        }
+        __syncthreads();
     }
 }
 
-// dweight and dbias: the per-sample channel sums added over the samples, in sample order per lane row
-static __global__ void gn_grad_params_kernel(const GnArgs a, const int chunks)
+template <typename T, int V>
+__global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_sums_kernel(const GnArgs a, const GnShape s)
 {
-    const int c = blockIdx.x * 32 + threadIdx.x;
-    const float2 *sums = gn_channel_sums(a, chunks);
+    gn_allow_second();
+    const GnPlace at(a, s, blockIdx.x);
+    const int count = at.count(s), c0 = at.vec * V;
+    constexpr int P = Pack<T, V>::P, U = kGnUnroll / 2;
+    __shared__ float2 acc[kGnThreads * V];                // [row slot][channel of the tile], then slot 0 the sums
+    {
+        const long long g0 = (long long)at.n * a.groups;
+        float2 mean[P], scale[P], bias[P], rstd[P], sgx[P], sg[P];
+        load_params<V>(a.weight, a.param_code, a.wide_params, c0, at.active, 1.0f, scale);
+        load_params<V>(a.bias, a.param_code, a.wide_params, c0, at.active, 0.0f, bias);
+        const int group = at.active ? c0 / a.cpg : at.group0, left = at.active ? (group + 1) * a.cpg - c0 : V;
+        spread_groups<V>(group, left, a.cpg, [&](int g) { return make_float2(-a.mean[g0 + g], a.rstd[g0 + g]); }, mean, rstd);
+#pragma unroll
+        for (int j = 0; j < P; ++j) { scale[j] = mul2(scale[j], rstd[j]); sgx[j] = sg[j] = both(0.0f); }
+        const long long first = (at.n * a.rows + at.row0 + at.r) * a.channels + c0, step = (long long)s.rows_per_step * a.channels;
+        const T *px = (const T *)a.x + first, *pd = (const T *)a.dy + first;
+        with_activation(a.act, [&](auto act) {
+            const auto add = [&](const Pack<T, V> &x, const Pack<T, V> &d) {
+                float2 f[P], z[P], g[P];
+                x.unpack(f);
+                d.unpack(g);
+#pragma unroll
+                for (int j = 0; j < P; ++j) { f[j] = add2(f[j], mean[j]); z[j] = fma2(f[j], scale[j], bias[j]); }
+                activate_grad<decltype(act)::value, sizeof(T) == 2, P>(z, g);
+#pragma unroll
+                for (int j = 0; j < P; ++j) { sg[j] = add2(sg[j], g[j]); sgx[j] = fma2(g[j], f[j], sgx[j]); }
+            };
+            Pack<T, V> x[U], d[U];
+            int i = 0;
+            for (; i + U <= count; i += U, px += U * step, pd += U * step) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) { x[u].load(px + u * step); d[u].load(pd + u * step); }
+#pragma unroll
+                for (int u = 0; u < U; ++u) add(x[u], d[u]);
+            }
+            for (; i < count; ++i, px += step, pd += step) {
+                x[0].load(px);
+                d[0].load(pd);
+                add(x[0], d[0]);
+            }
+        });
+        if (at.r < s.rows_per_step) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                acc[(at.r * s.tile + at.v) * V + j] = j % 2 ? make_float2(sgx[j / 2].y * rstd[j / 2].y, sg[j / 2].y)
+                                                            : make_float2(sgx[j / 2].x * rstd[j / 2].x, sg[j / 2].x);
+        }
+    }
+    __syncthreads();
+    const int tile_c0 = (at.vec - at.v) * V, channels = at.width(s) * V;
+    float2 *chan = a.channel_part + (long long)at.item * a.channels + tile_c0;
+    sum_columns(acc, s.tile * V, channels, s.rows_per_step, kGnThreads);
+    if (a.dweight || a.dbias)
+        for (int c = threadIdx.x; c < channels; c += kGnThreads) chan[c] = acc[c];
+    const int groups = at.groups(a, s), lanes = s.columns.lanes, lane = threadIdx.x & (lanes - 1), width = s.split == 1 ? a.cpg : channels;
+    for (int base = 0; base < groups; base += kGnThreads / lanes) {
+        const int g = base + threadIdx.x / lanes;
+        float ux = 0.0f, u = 0.0f;
+        if (g < groups)
+            for (int e = lane; e < width; e += lanes) {
+                const int c = g * width + e;
+                const float w = a.weight ? load_code(a.weight, a.param_code, tile_c0 + c) : 1.0f;
+                ux = fmaf(w, acc[c].x, ux);
+                u = fmaf(w, acc[c].y, u);
+            }
+        ux = lane_sum(ux, lanes);
+        u = lane_sum(u, lanes);
+        if (g < groups && lane == 0)
+            a.part[(((long long)at.n * a.groups + at.group0 + g) * s.chunks + at.chunk) * s.split + at.piece] = make_float2(ux, u);
+    }
+}
+
+// dweight and dbias of 32 channels: the channel sums of all samples and chunks, always added in the same order
+__device__ __forceinline__ void gn_param_grads(const GnArgs &a, const float2 *sums, long long rows, int block, float2 (*acc)[33])
+{
+    const int x = threadIdx.x % 32, y = threadIdx.x / 32, lanes = kGnThreads / 32, c = block * 32 + x;
     float gx = 0.0f, g = 0.0f;
-    if (c < a.channels)
-        for (long long n = threadIdx.y; n < a.n; n += blockDim.y) {
-            const float2 p = sums[n * a.channels + c];
+    if (c < a.channels) {
+#pragma unroll 8
+        for (long long i = y; i < rows; i += lanes) {
+            const float2 p = sums[i * a.channels + c];
             gx += p.x; g += p.y;
         }
-    __shared__ float2 acc[32][33];
-    acc[threadIdx.y][threadIdx.x] = make_float2(gx, g);
+    }
+    acc[y][x] = make_float2(gx, g);
     __syncthreads();
-    if (threadIdx.y == 0 && c < a.channels) {
+    if (y == 0 && c < a.channels) {
         gx = g = 0.0f;
-        for (int j = 0; j < (int)blockDim.y; ++j) { gx += acc[j][threadIdx.x].x; g += acc[j][threadIdx.x].y; }
+        for (int j = 0; j < lanes; ++j) { gx += acc[j][x].x; g += acc[j][x].y; }
         if (a.dweight) store_code(a.dweight, a.param_code, c, gx);
         if (a.dbias) store_code(a.dbias, a.param_code, c, g);
     }
 }
 
-// ----------------------------------------------------------------------------- launches
-template <typename T, int V> cudaError_t gn_launch_streaming(const GnArgs &a, bool backward, cudaStream_t stream)
+static __global__ void __launch_bounds__(kGnThreads) gn_grad_params_kernel(const GnArgs a, const float2 *sums, const long long rows)
 {
-    const GnShape s = gn_shape(a, V);
-    const dim3 grid((unsigned)(a.n * s.chunks), s.tiles);
-    const unsigned warps = (unsigned)((a.n * a.groups + 7) / 8);
-    if (!backward) {
-        gn_stats_kernel<T, V><<<grid, kGnThreads, 0, stream>>>(a, s);
-        gn_stats_finish_kernel<<<warps, 256, 0, stream>>>(a, s.chunks, s.chunk_rows);
-        gn_apply_kernel<T, V><<<grid, kGnThreads, 0, stream>>>(a, s);
-    } else {
-        gn_grad_sums_kernel<T, V><<<grid, kGnThreads, 0, stream>>>(a, s);
-        gn_grad_finish_kernel<<<warps, 256, 0, stream>>>(a, s.chunks);
-        if (a.dx) gn_grad_input_kernel<T, V><<<grid, kGnThreads, 0, stream>>>(a, s);
-        if (a.dweight || a.dbias)
-            gn_grad_params_kernel<<<(a.channels + 31) / 32, dim3(32, a.n >= 32 ? 32 : 8), 0, stream>>>(a, s.chunks);
+    __shared__ float2 acc[kGnThreads / 32][33];
+    gn_wait_first();
+    gn_param_grads(a, sums, rows, blockIdx.x, acc);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_input_kernel(const GnArgs a, const GnShape s)
+{
+    extern __shared__ float2 stat[];                      // [groups_per_tile] means of (u xhat, u)
+    const GnPlace at(a, s, gridDim.x - 1 - blockIdx.x);
+    const int count = at.count(s), c0 = at.vec * V;
+    constexpr int P = Pack<T, V>::P, U = kGnUnroll / 2;
+    const long long g0 = (long long)at.n * a.groups;
+    float2 mean[P], scale[P], bias[P], rstd[P], m_ux[P], m_u[P];
+    load_params<V>(a.weight, a.param_code, a.wide_params, c0, at.active, 1.0f, scale);
+    load_params<V>(a.bias, a.param_code, a.wide_params, c0, at.active, 0.0f, bias);
+    const int group = at.active ? c0 / a.cpg : at.group0, left = at.active ? (group + 1) * a.cpg - c0 : V;
+    spread_groups<V>(group, left, a.cpg, [&](int g) { return make_float2(-a.mean[g0 + g], a.rstd[g0 + g]); }, mean, rstd);
+#pragma unroll
+    for (int j = 0; j < P; ++j) scale[j] = mul2(scale[j], rstd[j]);
+    gn_wait_first();
+    const int groups = at.groups(a, s), lanes = s.finish_lanes, lane = threadIdx.x & (lanes - 1), entries = s.chunks * s.split;
+    const float inv = 1.0f / ((float)a.rows * (float)a.cpg);
+    for (int base = 0; base < groups; base += kGnThreads / lanes) {
+        const int g = base + threadIdx.x / lanes;
+        float ux = 0.0f, u = 0.0f;
+        if (g < groups) {
+            const float2 *part = a.part + ((long long)at.n * a.groups + at.group0 + g) * entries;
+#pragma unroll 4
+            for (int e = lane; e < entries; e += lanes) { const float2 p = __ldcg(part + e); ux += p.x; u += p.y; }
+        }
+        ux = lane_sum(ux, lanes);
+        u = lane_sum(u, lanes);
+        if (g < groups && lane == 0) stat[g] = make_float2(ux * inv, u * inv);
     }
-    return cudaGetLastError();
+    __syncthreads();
+    spread_groups<V>(group - at.group0, left, a.cpg, [&](int g) { return make_float2(-stat[g].x, -stat[g].y); }, m_ux, m_u);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {                         // dx = g scale - ((x - mean) m_ux + m_u)
+        m_ux[j] = mul2(m_ux[j], mul2(rstd[j], rstd[j]));
+        m_u[j] = mul2(m_u[j], rstd[j]);
+    }
+    const long long first = (at.n * a.rows + at.row0 + at.r) * a.channels + c0, step = (long long)s.rows_per_step * a.channels;
+    const T *px = (const T *)a.x + first, *pd = (const T *)a.dy + first;
+    T *out = (T *)a.dx + first;
+    with_activation(a.act, [&](auto act) {
+        const auto apply = [&](const Pack<T, V> &x, Pack<T, V> &d, T *to) {
+            float2 f[P], z[P], g[P];
+            x.unpack(f);
+            d.unpack(g);
+#pragma unroll
+            for (int j = 0; j < P; ++j) { f[j] = add2(f[j], mean[j]); z[j] = fma2(f[j], scale[j], bias[j]); }
+            activate_grad<decltype(act)::value, sizeof(T) == 2, P>(z, g);
+#pragma unroll
+            for (int j = 0; j < P; ++j) g[j] = fma2(g[j], scale[j], fma2(f[j], m_ux[j], m_u[j]));
+            d.pack(g);
+            d.store(to);
+        };
+        Pack<T, V> x[U], d[U];
+        int i = 0;
+        for (; i + U <= count; i += U, px += U * step, pd += U * step, out += U * step) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) { x[u].load_stream(px + u * step); d[u].load_stream(pd + u * step); }
+#pragma unroll
+            for (int u = 0; u < U; ++u) apply(x[u], d[u], out + u * step);
+        }
+        for (; i < count; ++i, px += step, pd += step, out += step) {
+            x[0].load_stream(px);
+            d[0].load_stream(pd);
+            apply(x[0], d[0], out);
+        }
+    });
+}
+
+// ----------------------------------------------------------------------------- launches
+template <typename Kernel, typename... Args>
+cudaError_t gn_launch_kernel(Kernel kernel, dim3 grid, size_t smem, bool dependent, cudaStream_t stream, Args... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kGnThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename T, int V> cudaError_t gn_launch_streaming(const GnArgs &all, bool backward, cudaStream_t stream)
+{
+    GnArgs a = all;
+    const GnShape s = gn_shape(a, V, backward);
+    const size_t smem = s.groups_per_tile * sizeof(float2);
+    const dim3 grid((unsigned)(a.n * s.chunks), s.tiles);
+    cudaError_t e;
+    if (!backward) {
+        e = gn_launch_kernel(gn_stats_kernel<T, V>, grid, 0, false, stream, a, s);
+        return e != cudaSuccess ? e : gn_launch_kernel(gn_apply_kernel<T, V>, grid, smem, true, stream, a, s);
+    }
+    a.channel_part = gn_channel_part(a, s);
+    e = gn_launch_kernel(gn_grad_sums_kernel<T, V>, grid, 0, false, stream, a, s);
+    if (e == cudaSuccess && a.dx) e = gn_launch_kernel(gn_grad_input_kernel<T, V>, grid, smem, true, stream, a, s);
+    if (e == cudaSuccess && (a.dweight || a.dbias))
+        e = gn_launch_kernel(gn_grad_params_kernel, dim3((a.channels + 31) / 32), 0, false, stream, a, (const float2 *)a.channel_part, a.n * s.chunks);
+    return e;
 }
 
 // Widest vector that divides the channels and that the pointers are aligned to
@@ -380,12 +716,22 @@ __host__ inline int gn_vector(const GnArgs &a, int elem_bytes)
     uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.dx;
     int v = 16 / elem_bytes;
     while (v > 1 && (a.channels % v != 0 || bits % (v * elem_bytes) != 0)) v /= 2;
+    while (v > 1 && gn_unit(a, v) > kGnThreads && a.cpg % v) v /= 2;
     return v;
 }
 
+}  // namespace ta
+
+#include "ta_group_norm_cluster.cuh"
+
+namespace ta {
+
 template <typename T> cudaError_t gn_launch(const GnArgs &a, bool backward, cudaStream_t stream)
 {
-    switch (gn_vector(a, sizeof(T))) {
+    const int v = gn_vector(a, sizeof(T));
+    GnPlan plan;
+    if (gn_plan(a, v, sizeof(T), backward, plan)) return gn_launch_planned<T>(a, plan, backward, stream);
+    switch (v) {
     case 8: if constexpr (sizeof(T) == 2) return gn_launch_streaming<T, 8>(a, backward, stream);
     case 4: return gn_launch_streaming<T, 4>(a, backward, stream);
     case 2: return gn_launch_streaming<T, 2>(a, backward, stream);

@@ -1,12 +1,15 @@
 #include "ta_group_norm.cuh"
 namespace ta {
 cudaError_t launch_group_norm_f32(const GnArgs &a, bool backward, cudaStream_t stream) { return gn_launch<float>(a, backward, stream); }
-}
-namespace ta {
-size_t group_norm_scratch_bytes(const GnArgs &a, int elem_bytes, bool backward)
+
+size_t group_norm_scratch_bytes(const GnArgs &all, int elem_bytes, bool backward)
 {
-    const GnShape s = gn_shape(a, gn_vector(a, elem_bytes));
-    const size_t rows = (size_t)a.n * (backward ? s.chunks + 1 : s.chunks);
-    return (rows * a.channels + (backward ? (size_t)a.n * a.groups : 0)) * sizeof(float2);
+    GnPlan plan;
+    if (gn_plan(all, gn_vector(all, elem_bytes), elem_bytes, backward, plan))
+        return backward && (all.dweight || all.dbias) ? (size_t)all.n * all.channels * sizeof(float2) : 0;
+    const GnShape s = gn_shape(all, gn_vector(all, elem_bytes), backward);
+    const size_t groups = (size_t)all.n * all.groups * s.chunks * s.split;
+    const size_t channels = backward && (all.dweight || all.dbias) ? (size_t)all.n * s.chunks * all.channels : 0;
+    return (groups + channels) * sizeof(float2);
 }
 }

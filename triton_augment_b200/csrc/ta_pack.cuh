@@ -41,30 +41,39 @@ template <typename T, int V> struct Pack {
     using Raw = typename RawOf<V * sizeof(T)>::type;
     union { Raw raw; T v[V]; typename FeatElem<T>::Pair p[V > 1 ? V / 2 : 1]; };
     __device__ __forceinline__ Pack() {}
+    __device__ __forceinline__ Pack(const Pack &o) : raw(o.raw) {}
+    __device__ __forceinline__ Pack &operator=(const Pack &o) { raw = o.raw; return *this; }
     __device__ __forceinline__ void load(const T *ptr) { raw = *reinterpret_cast<const Raw *>(ptr); }
     // read once, by this thread only: does not stay in the L1 cache
     __device__ __forceinline__ void load_stream(const T *ptr) { raw = __ldcs(reinterpret_cast<const Raw *>(ptr)); }
     __device__ __forceinline__ void store(T *ptr) const { *reinterpret_cast<Raw *>(ptr) = raw; }
-    __device__ __forceinline__ void unpack(float (&f)[V]) const
+    __device__ __forceinline__ void store_stream(T *ptr) const { __stcs(reinterpret_cast<Raw *>(ptr), raw); }
+    // as pairs of floats, the form of the packed arithmetic; a single element leaves its pair's second half 0
+    static constexpr int P = (V + 1) / 2;
+    __device__ __forceinline__ void unpack(float2 (&f)[P]) const
     {
-        if constexpr (V == 1) f[0] = FeatElem<T>::to_f(v[0]);
+        if constexpr (V == 1) f[0] = make_float2(FeatElem<T>::to_f(v[0]), 0.0f);
         else {
 #pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-                const float2 t = FeatElem<T>::to_f2(p[i]);
-                f[2 * i] = t.x; f[2 * i + 1] = t.y;
-            }
+            for (int i = 0; i < P; ++i) f[i] = FeatElem<T>::to_f2(p[i]);
         }
     }
-    __device__ __forceinline__ void pack(const float (&f)[V])
+    __device__ __forceinline__ void pack(const float2 (&f)[P])
     {
-        if constexpr (V == 1) v[0] = FeatElem<T>::from_f(f[0]);
+        if constexpr (V == 1) v[0] = FeatElem<T>::from_f(f[0].x);
         else {
 #pragma unroll
-            for (int i = 0; i < V / 2; ++i) p[i] = FeatElem<T>::from_f2(f[2 * i], f[2 * i + 1]);
+            for (int i = 0; i < P; ++i) p[i] = FeatElem<T>::from_f2(f[i].x, f[i].y);
         }
     }
 };
+
+// Two independent round-to-nearest operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 
 // Feature types by their TA_B200_* code (0 float32, 1 float16, 4 bfloat16), for operands that are read a few times per thread
 __device__ __forceinline__ float load_code(const void *p, int code, long long i)
