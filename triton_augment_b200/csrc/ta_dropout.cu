@@ -21,53 +21,178 @@ __device__ __forceinline__ uint4 mask_words(uint2 key, unsigned long long block,
     return philox4x32_10(key, make_uint4((uint32_t)block, (uint32_t)(block >> 32), offset, tag));
 }
 
-__device__ __forceinline__ uint32_t half_of(const uint4 &w, int slot)
+__device__ __forceinline__ uint32_t word_of(const uint4 &w, int i) { return i < 2 ? (i == 0 ? w.x : w.y) : (i == 2 ? w.z : w.w); }
+
+// Bit j: entry 8 block + j is kept
+__device__ __forceinline__ uint32_t keep_bits(const DropoutArgs &a, uint2 key, unsigned long long block)
 {
-    const uint32_t word = slot < 4 ? (slot < 2 ? w.x : w.y) : (slot < 6 ? w.z : w.w);
-    return slot & 1 ? word >> 16 : word & 0xFFFFu;
+    const uint4 w = mask_words(key, block, a.offset, kDropoutTag);
+    const uint32_t upper = a.thr_hi << 16;
+    uint32_t bits = 0, equal = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t v = word_of(w, i);
+        if ((v << 16) >= upper) bits |= 1u << (2 * i);
+        if (v >= upper) bits |= 2u << (2 * i);
+        // a half of v equal to the threshold (or, harmlessly, its neighbour): the test for zero bytes, on halves
+        const uint32_t t = v ^ (upper | a.thr_hi);
+        equal |= (t - 0x00010001u) & ~t & 0x80008000u;
+    }
+    if (a.thr_lo != 0 && equal != 0) {
+        const uint4 lo = mask_words(key, block, a.offset, kDropoutTag + 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t v = word_of(w, i), l = word_of(lo, i);
+            if ((v & 0xFFFFu) == a.thr_hi && (l & 0xFFFFu) < a.thr_lo) bits &= ~(1u << (2 * i));
+            if ((v >> 16) == a.thr_hi && (l >> 16) < a.thr_lo) bits &= ~(2u << (2 * i));
+        }
+    }
+    return bits;
 }
 
-// One mask entry on its own
-__device__ __forceinline__ bool keep_entry(const DropoutArgs &a, uint2 key, unsigned long long entry)
+// Bit j: mask entry m + j is kept (eight entries in a row, from one block or two)
+__device__ __forceinline__ uint32_t keep_run(const DropoutArgs &a, uint2 key, unsigned long long m)
 {
-    const int slot = (int)(entry & 7);
-    const uint32_t hi = half_of(mask_words(key, entry >> 3, a.offset, kDropoutTag), slot);
-    if (hi != a.thr_hi) return hi > a.thr_hi;
-    return half_of(mask_words(key, entry >> 3, a.offset, kDropoutTag + 1), slot) >= a.thr_lo;
+    const int shift = (int)(m & 7);
+    uint32_t bits = keep_bits(a, key, m >> 3);
+    if (shift) bits = (bits | keep_bits(a, key, (m >> 3) + 1) << 8) >> shift;
+    return bits & 0xFFu;
 }
 
-__device__ __forceinline__ unsigned long long mask_index(const DropoutArgs &a, unsigned long long e)
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv &f)
+{
+    const uint32_t t = __umulhi(n, f.m);
+    return (t + ((n - t) >> f.s1)) >> f.s2;
+}
+
+// Mask entry of element e; with `rest`, how many elements follow in the innermost dimension
+__device__ __forceinline__ unsigned long long mask_index(const DropoutArgs &a, unsigned long long e, long long *rest = nullptr)
 {
     unsigned long long m = 0;
 #pragma unroll
     for (int d = 3; d >= 0; --d) {
-        const unsigned long long q = e / (unsigned long long)a.size[d];
-        m += (e - q * a.size[d]) * a.mstride[d];
+        const unsigned long long q = e / (unsigned long long)a.size[d], c = e - q * a.size[d];
+        if (d == 3 && rest) *rest = a.size[3] - (long long)c;
+        m += c * a.mstride[d];
+        e = q;
+    }
+    return m;
+}
+__device__ __forceinline__ unsigned long long mask_index32(const DropoutArgs &a, uint32_t e, long long *rest)
+{
+    unsigned long long m = 0;
+#pragma unroll
+    for (int d = 3; d >= 0; --d) {
+        if (d < 3 && a.size[d] == 1) continue;
+        const uint32_t q = d == 0 ? 0 : fast_div(e, a.div[d]), c = d == 0 ? e : e - q * a.div[d].d;
+        if (d == 3) *rest = a.size[3] - (long long)c;
+        m += (unsigned long long)c * a.mstride[d];
         e = q;
     }
     return m;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kDropoutThreads) dropout_kernel(const DropoutArgs a)
+enum { kMaskLinear = 0, kMask32 = 1, kMask64 = 2 };       // entry = element; dimensions of fewer than 2^32 elements; any
+
+// Bit j: element e + j is kept, j < 8
+template <int KIND> __device__ __forceinline__ uint32_t keep_elements(const DropoutArgs &a, uint2 key, long long e, int valid)
 {
+    if (a.drop_all) return 0;
+    if constexpr (KIND == kMaskLinear) return keep_bits(a, key, (unsigned long long)e >> 3);
+    long long rest;
+    const unsigned long long m = KIND == kMask32 ? mask_index32(a, (uint32_t)e, &rest) : mask_index(a, e, &rest);
+    if (rest >= 8) {                                      // eight neighbours in a row: one entry for all, or eight in a row
+        if (a.mstride[3] != 0) return keep_run(a, key, m);
+        return (keep_bits(a, key, m >> 3) >> (m & 7)) & 1u ? 0xFFu : 0u;
+    }
+    uint32_t out = 0, bits = 0;
+    unsigned long long have = ~0ull;
+    for (int j = 0; j < valid; ++j) {
+        long long r;
+        const unsigned long long mj = KIND == kMask32 ? mask_index32(a, (uint32_t)(e + j), &r) : mask_index(a, e + j, &r);
+        if (mj >> 3 != have) {
+            have = mj >> 3;
+            bits = keep_bits(a, key, have);
+        }
+        out |= ((bits >> (mj & 7)) & 1u) << j;
+    }
+    return out;
+}
+
+// Every thread: U times eight elements, their loads first; the generator's work hides the loads' latency.
+// WIDE: all tensors on 16-byte boundaries.
+template <typename T, int KIND, bool WIDE, bool RESIDUAL>
+__global__ void __launch_bounds__(kDropoutThreads) dropout_kernel(const __grid_constant__ DropoutArgs a)
+{
+    constexpr int V = 16 / sizeof(T), N = 8 / V, U = sizeof(T) == 2 ? 2 : 1;      // N vectors of 16 bytes are eight elements
     const uint64_t seed = a.seed_ptr ? *a.seed_ptr : a.seed;
     const uint2 key = make_uint2((uint32_t)seed, (uint32_t)(seed >> 32));
-    const long long step = (long long)gridDim.x * kDropoutThreads;
-    for (long long e = (long long)blockIdx.x * kDropoutThreads + threadIdx.x; e < a.numel; e += step) {
-        const float x = FeatElem<T>::to_f(((const T *)a.x)[e]);
-        float y = keep_entry(a, key, mask_index(a, e)) ? x * a.scale : 0.0f;
-        if (a.residual) y += FeatElem<T>::to_f(((const T *)a.residual)[e]);
-        ((T *)a.y)[e] = FeatElem<T>::from_f(y);
+    const T *px = (const T *)a.x, *pr = (const T *)a.residual;
+    T *py = (T *)a.y;
+    const long long first = ((long long)blockIdx.x * U * kDropoutThreads + threadIdx.x) * 8;
+    Pack<T, V> x[U][N], r[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long e = first + (long long)u * kDropoutThreads * 8;
+        if (WIDE && e + 8 <= a.numel) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                x[u][i].load_stream(px + e + i * V);
+                if (RESIDUAL) r[u][i].load_stream(pr + e + i * V);
+            }
+        }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long e = first + (long long)u * kDropoutThreads * 8;
+        if (e >= a.numel) break;
+        const int valid = (int)min(8LL, a.numel - e);
+        const uint32_t keep = keep_elements<KIND>(a, key, e, valid);
+        if (WIDE && valid == 8) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float2 f[V / 2], g[V / 2];
+                x[u][i].unpack(f);
+                if (RESIDUAL) r[u][i].unpack(g);
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    const uint32_t b = keep >> (i * V + 2 * j);
+                    // a dropped element contributes 0 whatever it holds: selected, not multiplied
+                    f[j] = make_float2(b & 1u ? f[j].x * a.scale : 0.0f, b & 2u ? f[j].y * a.scale : 0.0f);
+                    if (RESIDUAL) f[j] = add2(f[j], g[j]);
+                }
+                x[u][i].pack(f);
+                x[u][i].store(py + e + i * V);
+            }
+        } else {
+            for (int j = 0; j < valid; ++j) {
+                float f = (keep >> j) & 1u ? FeatElem<T>::to_f(px[e + j]) * a.scale : 0.0f;
+                if (RESIDUAL) f += FeatElem<T>::to_f(pr[e + j]);
+                py[e + j] = FeatElem<T>::from_f(f);
+            }
+        }
+    }
+}
+
+template <typename T, int KIND> static cudaError_t dropout_launch_kind(const DropoutArgs &a, cudaStream_t stream)
+{
+    constexpr int per_block = kDropoutThreads * 8 * (sizeof(T) == 2 ? 2 : 1);
+    const unsigned blocks = (unsigned)((a.numel + per_block - 1) / per_block);
+    const bool wide = (((uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.residual) % 16) == 0;
+    if (a.residual) {
+        if (wide) dropout_kernel<T, KIND, true, true><<<blocks, kDropoutThreads, 0, stream>>>(a);
+        else dropout_kernel<T, KIND, false, true><<<blocks, kDropoutThreads, 0, stream>>>(a);
+    } else {
+        if (wide) dropout_kernel<T, KIND, true, false><<<blocks, kDropoutThreads, 0, stream>>>(a);
+        else dropout_kernel<T, KIND, false, false><<<blocks, kDropoutThreads, 0, stream>>>(a);
+    }
+    return cudaGetLastError();
 }
 
 template <typename T> static cudaError_t dropout_launch(const DropoutArgs &a, cudaStream_t stream)
 {
-    long long blocks = (a.numel + kDropoutThreads - 1) / kDropoutThreads;
-    if (blocks > 8LL * a.sm_count) blocks = 8LL * a.sm_count;
-    dropout_kernel<T><<<(unsigned)blocks, kDropoutThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+    if (a.size[3] == a.numel && a.mstride[3] == 1) return dropout_launch_kind<T, kMaskLinear>(a, stream);
+    return a.numel < (1LL << 32) ? dropout_launch_kind<T, kMask32>(a, stream) : dropout_launch_kind<T, kMask64>(a, stream);
 }
 
 cudaError_t launch_dropout(const DropoutArgs &a, int dtype, cudaStream_t stream)
