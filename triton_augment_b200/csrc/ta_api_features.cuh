@@ -150,8 +150,8 @@ static int rotary(const ta_b200_rotary_params *p, cudaStream_t stream)
     }
     if (rot > p->dim) return fail(TA_B200_ERR_SHAPE, "sections add up to more than the head dimension %d", p->dim);
     if (rot / 2 > kRotaryMaxPairs) return fail(TA_B200_ERR_TOO_LARGE, "at most %d rotated elements per head", 2 * kRotaryMaxPairs);
-    if (p->dim > 65536 || p->q_heads > 65536 || p->k_heads > 65536 || (double)p->n * p->tokens * p->dim >= 1.0e15)
-        return fail(TA_B200_ERR_TOO_LARGE, "head dimension and heads up to 65536");
+    if (p->tokens >= (1LL << 31) || p->dim > 65536 || p->q_heads > 65536 || p->k_heads > 65536 || (double)p->n * p->tokens * p->dim >= 1.0e15)
+        return fail(TA_B200_ERR_TOO_LARGE, "tokens below 2^31, head dimension and heads up to 65536");
     if (!(p->base > 0.0)) return fail(TA_B200_ERR_UNSUPPORTED, "base must be positive");
     if (p->pairing != TA_B200_PAIR_INTERLEAVED && p->pairing != TA_B200_PAIR_HALVES) return fail(TA_B200_ERR_UNSUPPORTED, "pairing %d", p->pairing);
     if (p->spectrum != TA_B200_SPECTRUM_AXIS && p->spectrum != TA_B200_SPECTRUM_JOINT)
@@ -189,6 +189,8 @@ static int rotary(const ta_b200_rotary_params *p, cudaStream_t stream)
         a.pos_s[i] = p->position_strides[i];
         a.grid[i] = p->grid[i] > 0 ? p->grid[i] : 1;
     }
+    for (int i = 0; i < 3; ++i) a.grid_div[i] = fast_div_of((uint32_t)a.grid[i]);
+    a.token_div = fast_div_of((uint32_t)p->tokens);
     a.n = p->n; a.tokens = p->tokens; a.prefix = p->prefix; a.q_heads = p->q_heads; a.k_heads = p->k_heads; a.dim = p->dim;
     a.axes = p->axes; a.pairs = rot / 2; a.halves = p->pairing == TA_B200_PAIR_HALVES; a.inverse = p->inverse != 0;
     a.pos_kind = p->position_kind; a.positions = p->positions; a.patch = p->patch;

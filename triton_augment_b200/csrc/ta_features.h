@@ -72,6 +72,7 @@ struct RotaryArgs {
     const void *positions;
     long long pos_s[3];                          // element strides of sample, token, axis
     int grid[3];
+    FastDiv grid_div[3], token_div;              // token_div: of tokens
     float patch;
     const float *top, *left;
     const uint8_t *flip;

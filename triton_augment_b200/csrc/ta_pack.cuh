@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "ta_features.h"
+
 namespace ta {
 
 template <typename T> struct FeatElem;
@@ -74,6 +76,12 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
 __device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv &f)
+{
+    const uint32_t t = __umulhi(n, f.m);
+    return (t + ((n - t) >> f.s1)) >> f.s2;
+}
 
 // Feature types by their TA_B200_* code (0 float32, 1 float16, 4 bfloat16), for operands that are read a few times per thread
 __device__ __forceinline__ float load_code(const void *p, int code, long long i)

@@ -29,33 +29,41 @@ __device__ __forceinline__ void cos_sin_of(const AxisPos &p, float fh, float fl,
     if (inverse) s = -s;
 }
 
-// position of token l (counted after the prefix) of sample n on axis `axis`
-__device__ __forceinline__ AxisPos axis_position(const RotaryArgs &a, long long n, long long l, int axis)
+// positions of token l (counted after the prefix) of sample n on its axes
+__device__ __forceinline__ void axis_positions(const RotaryArgs &a, long long n, int l, AxisPos (&pos)[3])
 {
-    AxisPos r;
-    r.lo = 0.0f;
+#pragma unroll
+    for (int d = 0; d < 3; ++d) pos[d] = {0.0f, 0.0f};
     if (a.pos_kind == 0) {
-        long long i = l;
-        for (int d = a.axes - 1; d > axis; --d) i /= a.grid[d];
-        i %= a.grid[axis];
-        const bool column = axis == a.axes - 1;
-        if (column && a.flip && a.flip[n]) i = a.grid[axis] - 1 - i;
-        // in pixels (the frequencies are per pixel): offset of the window + patch x index, as an exact sum of two floats
-        const float step = (float)i * a.patch;
-        const float origin = column ? (a.left ? a.left[n] : 0.0f) : axis == a.axes - 2 && a.top ? a.top[n] : 0.0f;
-        r.hi = origin + step;
-        const float b = r.hi - origin;
-        r.lo = (origin - (r.hi - b)) + (step - b);
-        return r;
+        uint32_t left = (uint32_t)l;
+#pragma unroll
+        for (int d = 2; d >= 0; --d) {
+            if (d >= a.axes) continue;
+            const uint32_t q = d == 0 ? 0u : fast_div(left, a.grid_div[d]);
+            int i = (int)(left - q * (uint32_t)a.grid[d]);
+            left = q;
+            float origin = 0.0f;
+            if (d == a.axes - 1) {
+                if (a.flip && a.flip[n]) i = a.grid[d] - 1 - i;
+                if (a.left) origin = a.left[n];
+            } else if (d == a.axes - 2 && a.top) origin = a.top[n];
+            // in pixels (the frequencies are per pixel): offset of the window + patch x index, as an exact sum of two floats
+            const float step = (float)i * a.patch, sum = origin + step, b = sum - origin;
+            pos[d] = {sum, (origin - (sum - b)) + (step - b)};
+        }
+        return;
     }
-    const long long at = n * a.pos_s[0] + (l + a.prefix) * a.pos_s[1] + axis * a.pos_s[2];
-    if (a.pos_kind == 2) { r.hi = ((const float *)a.positions)[at]; return r; }
-    const long long p = a.pos_kind == 1 ? ((const long long *)a.positions)[at] : (long long)((const int *)a.positions)[at];
-    const long long low = p & 0xFFFFFF;                 // two exact floats up to 2^48
-    r.hi = (float)(p - low);
-    r.lo = (float)low;
-    if (r.hi == 0.0f) { r.hi = r.lo; r.lo = 0.0f; }
-    return r;
+    const long long at = n * a.pos_s[0] + (long long)(l + a.prefix) * a.pos_s[1];
+#pragma unroll
+    for (int d = 0; d < 3; ++d) {
+        if (d >= a.axes) continue;
+        const long long i = at + d * a.pos_s[2];
+        if (a.pos_kind == 2) { pos[d].hi = ((const float *)a.positions)[i]; continue; }
+        const long long p = a.pos_kind == 1 ? ((const long long *)a.positions)[i] : (long long)((const int *)a.positions)[i];
+        const long long low = p & 0xFFFFFF;               // two exact floats up to 2^48
+        pos[d] = {(float)(p - low), (float)low};
+        if (pos[d].hi == 0.0f) pos[d] = {pos[d].lo, 0.0f};
+    }
 }
 
 // ----------------------------------------------------------------------------- scalar kernel
@@ -73,7 +81,9 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_scalar_kernel(const __g
         float c = 1.0f, s = 0.0f;
         if (turn) {
             const int axis = u < a.axis_end[0] ? 0 : u < a.axis_end[1] ? 1 : 2;
-            cos_sin_of(axis_position(a, n, l - a.prefix, axis), a.freq_hi[u], a.freq_lo[u], a.inverse, c, s);
+            AxisPos pos[3];
+            axis_positions(a, n, (int)l - a.prefix, pos);
+            cos_sin_of(axis == 0 ? pos[0] : axis == 1 ? pos[1] : pos[2], a.freq_hi[u], a.freq_lo[u], a.inverse, c, s);
         }
         const int i0 = pair ? (a.halves ? u : 2 * u) : a.pairs + u, i1 = pair ? (a.halves ? u + a.pairs : 2 * u + 1) : i0;
         for (int h = 0; h < a.q_heads + a.k_heads; ++h) {
@@ -117,7 +127,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
     if (tl >= p.block_tokens || u >= p.units) return;
     const bool turned = u < p.turned;
     // element offsets of the vector(s); behind the rotated part there is one vector to a unit
-    const int i0 = !HALVES ? u * V : turned ? u * V : 2 * a.pairs + (u - p.turned) * V, i1 = i0 + a.pairs;
+    const int i0 = !HALVES ? u * V : turned ? u * V : 2 * a.pairs + (u - p.turned) * V;
     float fh[PAIRS], fl[PAIRS];
     int axis_of[PAIRS];
     if (turned) {
@@ -132,19 +142,19 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
     const int heads = a.q_heads + a.k_heads;
     const long long tokens = a.n * a.tokens;
     for (long long tok = (long long)blockIdx.x * p.block_tokens + tl; tok < tokens; tok += (long long)gridDim.x * p.block_tokens) {
-        const long long n = tokens < (1LL << 32) ? (uint32_t)tok / (uint32_t)a.tokens : tok / a.tokens, l = tok - n * a.tokens;
+        const long long n = tokens < (1LL << 32) ? fast_div((uint32_t)tok, a.token_div) : tok / a.tokens;
+        const int l = (int)(tok - n * a.tokens);
         const bool turn = turned && l >= a.prefix;
+        const T *q = (const T *)a.q + n * a.qs[0] + l * a.qs[1] + i0, *k = (const T *)a.k + n * a.ks[0] + l * a.ks[1] + i0;
+        T *qo = (T *)a.q_out + n * a.qos[0] + l * a.qos[1] + i0, *ko = (T *)a.k_out + n * a.kos[0] + l * a.kos[1] + i0;
         float c[PAIRS], s[PAIRS];
         if (turn) {
             AxisPos pos[3];
-#pragma unroll
-            for (int d = 0; d < 3; ++d) pos[d] = d < a.axes ? axis_position(a, n, l - a.prefix, d) : AxisPos{0.0f, 0.0f};
+            axis_positions(a, n, l - a.prefix, pos);
 #pragma unroll
             for (int j = 0; j < PAIRS; ++j)
                 cos_sin_of(axis_of[j] == 0 ? pos[0] : axis_of[j] == 1 ? pos[1] : pos[2], fh[j], fl[j], a.inverse, c[j], s[j]);
         }
-        const T *q = (const T *)a.q + n * a.qs[0] + l * a.qs[1], *k = (const T *)a.k + n * a.ks[0] + l * a.ks[1];
-        T *qo = (T *)a.q_out + n * a.qos[0] + l * a.qos[1], *ko = (T *)a.k_out + n * a.kos[0] + l * a.kos[1];
         for (int h0 = hg; h0 < heads; h0 += kRotaryBatch * p.head_step) {
             Pack<T, V> x[kRotaryBatch], y[HALVES ? kRotaryBatch : 1];
 #pragma unroll
@@ -152,8 +162,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
                 const int h = h0 + b * p.head_step;
                 if (h >= heads) continue;
                 const T *in = h < a.q_heads ? q + h * a.qs[2] : k + (h - a.q_heads) * a.ks[2];
-                x[b].load_stream(in + i0);
-                if (HALVES && turned) y[b].load_stream(in + i1);
+                x[b].load_stream(in);
+                if (HALVES && turned) y[b].load_stream(in + a.pairs);
             }
 #pragma unroll
             for (int b = 0; b < kRotaryBatch; ++b) {
@@ -179,8 +189,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
                     x[b].pack(f);
                 }
                 T *out = h < a.q_heads ? qo + h * a.qos[2] : ko + (h - a.q_heads) * a.kos[2];
-                x[b].store(out + i0);
-                if (HALVES && turned) y[b].store(out + i1);
+                x[b].store(out);
+                if (HALVES && turned) y[b].store(out + a.pairs);
             }
         }
     }
@@ -196,9 +206,10 @@ template <typename T, int V, bool HALVES> static cudaError_t rotary_launch_vecto
     p.unit_blocks = (p.units + p.block_units - 1) / p.block_units;
     const long long tokens = a.n * a.tokens;
     // As few threads per token as still fill the GPU, so that a thread's cosines serve many heads: they cost as much
-    // as about five heads' rotations.  Single tokens get a thread per head.
-    const long long fill = (long long)a.sm_count * 1024;
-    int step = (heads + 2 * kRotaryBatch - 1) / (2 * kRotaryBatch);
+    // as about five heads' rotations (16 x 4096 tokens x 32 heads x 128, 4 / 8 / 16 / 32 heads to a thread: 217 / 189 /
+    // 182 / 190 us).  Single tokens get a thread per head.
+    const long long fill = (long long)a.sm_count * 512;
+    int step = (heads + 15) / 16;
     while (step < heads && tokens * p.units * step < fill) step = step * 2 < heads ? step * 2 : heads;
     if (step > kRotaryThreads / p.block_units) step = kRotaryThreads / p.block_units;
     p.head_step = step < 1 ? 1 : step;
