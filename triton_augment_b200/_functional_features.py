@@ -12,7 +12,7 @@ of the eager call.
 """
 from __future__ import annotations
 
-import ctypes as C
+import math
 
 import torch
 
@@ -55,59 +55,61 @@ def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def _address(t):
-    return None if t is None else t.data_ptr()
+def _address(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _channels_last(t):
+    """``t`` with its channels (dimension -3) last in memory and no gaps; ``t`` itself if it is already."""
+    if t.ndim == 4:
+        return t.contiguous(memory_format=torch.channels_last)
+    last = t.movedim(-3, -1)
+    return t if last.is_contiguous() else last.contiguous().movedim(-1, -3)
 
 
 # ----------------------------------------------------------------------------- group norm
-def _group_norm_params(xm, weight, bias, groups, eps, act, samples) -> "_lib.GroupNormParams":
-    p = _lib.GroupNormParams()
-    p.struct_size = C.sizeof(_lib.GroupNormParams)
-    p.dtype = _lib.FEATURE_CODES[xm.dtype]
-    param = weight if weight is not None else bias
-    p.param_dtype = _lib.F32 if param is None else _lib.FEATURE_CODES[param.dtype]
-    p.activation = act
-    channels = xm.shape[-1]
-    p.n, p.rows = samples, (xm.numel() // (samples * channels) if samples else 0)
-    p.channels, p.groups, p.eps = channels, groups, eps
-    p.x, p.weight, p.bias = xm.data_ptr(), _address(weight), _address(bias)
-    return p
+def _group_norm_fields(x, param, groups, eps, act, samples):
+    """Fields of ta_b200_group_norm_params up to eps (and the padding behind it)."""
+    channels, numel = x.shape[-3], x.numel()
+    return (_lib.FEATURE_CODES[x.dtype], _lib.F32 if param is None else _lib.FEATURE_CODES[param.dtype], act,
+            samples, numel // (samples * channels) if samples else 0, channels, groups, eps, 0)
 
 
 def _group_norm_forward(x, weight, bias, groups, eps, act, samples):
-    """Features with channels last in memory, the result, and the statistics [2, samples * groups]."""
-    xm = x.movedim(-3, -1).contiguous()
-    y = torch.empty_like(xm)
-    stats = torch.empty(2, samples * groups, dtype=torch.float32, device=x.device)
-    p = _group_norm_params(xm, weight, bias, groups, eps, act, samples)
-    p.y, p.mean, p.rstd = y.data_ptr(), stats.data_ptr(), stats.data_ptr() + 4 * samples * groups
-    _lib.launch_group_norm(p, x.device)
-    return xm, y.movedim(-1, -3), stats
+    """The features with channels last in memory, the result, and the statistics [2, samples * groups]."""
+    x = _channels_last(x)
+    y = torch.empty_like(x)
+    stats = torch.empty(2 * samples * groups, dtype=torch.float32, device=x.device)
+    mean = stats.data_ptr()
+    fields = _group_norm_fields(x, bias if weight is None else weight, groups, eps, act, samples)
+    _lib.launch_group_norm(fields + (x.data_ptr(), _address(weight), _address(bias), y.data_ptr(), mean, mean + 4 * samples * groups,
+                                     0, 0, 0, 0), x.device)
+    return x, y, stats
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act, samples):
-        xm, y, stats = _group_norm_forward(x, weight, bias, groups, eps, act, samples)
-        ctx.save_for_backward(xm, weight, bias, stats)
+        x, y, stats = _group_norm_forward(x, weight, bias, groups, eps, act, samples)
+        ctx.save_for_backward(x, weight, bias, stats)
         ctx.rest = (groups, eps, act, samples)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        xm, weight, bias, stats = ctx.saved_tensors
+        x, weight, bias, stats = ctx.saved_tensors
         groups, eps, act, samples = ctx.rest
-        dym = dy.movedim(-3, -1).contiguous()
-        p = _group_norm_params(xm, weight, bias, groups, eps, act, samples)
-        p.mean, p.rstd = stats.data_ptr(), stats.data_ptr() + 4 * samples * groups
-        p.dy = dym.data_ptr()
-        dx = torch.empty_like(xm) if ctx.needs_input_grad[0] else None
-        dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
-        db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
-        p.dx, p.dweight, p.dbias = _address(dx), _address(dw), _address(db)
-        _lib.launch_group_norm(p, xm.device, backward=True)
-        return None if dx is None else dx.movedim(-1, -3), dw, db, None, None, None, None
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        dy = _channels_last(dy)
+        dx = torch.empty_like(x) if want_x else None
+        dw = torch.empty_like(weight) if want_w else None
+        db = torch.empty_like(bias) if want_b else None
+        mean = stats.data_ptr()
+        fields = _group_norm_fields(x, bias if weight is None else weight, groups, eps, act, samples)
+        _lib.launch_group_norm(fields + (x.data_ptr(), _address(weight), _address(bias), 0, mean, mean + 4 * samples * groups,
+                                         dy.data_ptr(), _address(dx), _address(dw), _address(db)), x.device, backward=True)
+        return dx, dw, db, None, None, None, None
 
 
 def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5, activation: str = "none", *,
@@ -155,20 +157,22 @@ _MODES = {"element": 0, "channel": 1, "pixel": 2, "sample": 3}
 
 
 def _memory_order(x):
-    """``x`` dense in memory order, and whether that order has the channels last."""
+    """``x`` without gaps, row-major or with its channels last, and whether it is the latter."""
     if x.is_contiguous():
         return x, False
-    if x.ndim in (3, 4, 5):
-        last = x.movedim(-3, -1)
-        if last.is_contiguous():
-            return last, True
+    if x.ndim in (3, 4, 5) and x.movedim(-3, -1).is_contiguous():
+        return x, True
     return x.contiguous(), False
+
+
+def _in_order(t, last):
+    return _channels_last(t) if last else t.contiguous()
 
 
 def _mask_layout(shape, channels_last, mode, same_on_batch, same_on_frame):
     """Four sizes of the tensor in memory order and the bit set of those the mask is shared along."""
     if mode == 0 and not (same_on_batch or same_on_frame):
-        return (1, 1, 1, torch.Size(shape).numel()), 0
+        return (1, 1, 1, math.prod(shape)), 0
     n = shape[0] if len(shape) >= 4 else 1
     t = shape[1] if len(shape) == 5 else 1
     c, plane = shape[-3], shape[-2] * shape[-1]
@@ -178,26 +182,20 @@ def _mask_layout(shape, channels_last, mode, same_on_batch, same_on_frame):
     return ((n, t, plane, c) if channels_last else (n, t, c, plane)), shared
 
 
-def _dropout_launch(xm, residual, layout, p, seed, seed_tensor, offset):
-    y = torch.empty_like(xm)
-    a = _lib.DropoutParams()
-    a.struct_size = C.sizeof(_lib.DropoutParams)
-    a.dtype = _lib.FEATURE_CODES[xm.dtype]
-    a.sizes[:], a.shared = layout
-    a.offset, a.p, a.seed = offset, p, seed
-    a.seed_ptr = _address(seed_tensor)
-    a.x, a.residual, a.y = xm.data_ptr(), _address(residual), y.data_ptr()
-    _lib.launch_dropout(a, xm.device)
+def _dropout_launch(x, residual, layout, p, seed, seed_tensor, offset):
+    y = torch.empty_like(x)
+    sizes, shared = layout
+    _lib.launch_dropout((_lib.FEATURE_CODES[x.dtype], *sizes, shared, offset, p, seed, _address(seed_tensor), x.data_ptr(),
+                         _address(residual), y.data_ptr()), x.device)
     return y
 
 
 def _dropout_forward(x, residual, p, seed, seed_tensor, offset, mode, same_on_batch, same_on_frame):
-    xm, last = _memory_order(x)
+    x, last = _memory_order(x)
     layout = _mask_layout(x.shape, last, mode, same_on_batch, same_on_frame)
     if residual is not None:
-        residual = (residual.movedim(-3, -1) if last else residual).contiguous()
-    y = _dropout_launch(xm, residual, layout, p, seed, seed_tensor, offset)
-    return (y.movedim(-1, -3) if last else y), last, layout
+        residual = _in_order(residual, last)
+    return _dropout_launch(x, residual, layout, p, seed, seed_tensor, offset), last, layout
 
 
 class _Dropout(torch.autograd.Function):
@@ -215,8 +213,7 @@ class _Dropout(torch.autograd.Function):
         last, layout, p, seed, offset = ctx.rest
         dx = None
         if ctx.needs_input_grad[0]:
-            dx = _dropout_launch((dy.movedim(-3, -1) if last else dy).contiguous(), None, layout, p, seed, seed_tensor, offset)
-            dx = dx.movedim(-1, -3) if last else dx
+            dx = _dropout_launch(_in_order(dy, last), None, layout, p, seed, seed_tensor, offset)
         return (dx, dy if ctx.needs_input_grad[1] else None) + (None,) * 7
 
 
@@ -279,52 +276,81 @@ def dropout(x, p: float = 0.5, seed=None, *, offset: int = 0, mode: str = "eleme
 
 # ----------------------------------------------------------------------------- rotary positions
 class _Rotary:
-    """The part of a call that forward and backward share."""
-    __slots__ = ("sections", "base", "pairing", "spectrum", "prefix", "grid", "patch")
+    """What of a call does not depend on its tensors, checked and laid out once per configuration."""
+    __slots__ = ("sections", "grid", "prefix", "head", "middle", "tail")
+
+    def __init__(self, sections, grid, patch, base, pairing, spectrum, prefix):
+        self.sections = tuple(int(s) for s in sections)
+        axes = len(self.sections)
+        if not 1 <= axes <= 3:
+            raise ValueError(f"sections must name one to three axes, got {axes}")
+        if any(s < 0 or s % 2 for s in self.sections) or sum(self.sections) > 512:
+            raise ValueError(f"sections must be even, not negative, and add up to at most 512, got {self.sections}")
+        base = float(base)
+        if not 0.0 < base < float("inf"):
+            raise ValueError(f"base must be positive, got {base}")
+        pairing, spectrum = _choice(pairing, _lib.PAIRINGS, "pairing"), _choice(spectrum, _lib.SPECTRA, "spectrum")
+        self.prefix = int(prefix)
+        self.grid = None
+        patch = float(patch)
+        if grid is not None:
+            self.grid = tuple(int(g) for g in grid)
+            if len(self.grid) != axes or any(g < 0 for g in self.grid):
+                raise ValueError(f"grid must have {axes} sizes like sections, got {grid}")
+            if not 0.0 < patch < float("inf"):
+                raise ValueError(f"patch must be positive, got {patch}")
+        pad = (0,) * (3 - axes)
+        # ta_b200_rotary_params: axes, sections, pairing, spectrum | base | grid, patch
+        self.head = (axes, *self.sections, *pad, pairing, spectrum)
+        self.middle = base
+        self.tail = ((0, 0, 0) if grid is None else self.grid + pad) + (patch,)
+
+
+_ROTARY_CACHE = {}
+
+
+def _rotary_spec(*key) -> _Rotary:
+    spec = _ROTARY_CACHE.get(key)
+    if spec is None:
+        spec = _Rotary(*key)
+        if len(_ROTARY_CACHE) < 64:
+            _ROTARY_CACHE[key] = spec
+    return spec
 
 
 def _inner_dense(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+_ABSENT = (0, 0, 0)
+
+
 def _rotary_launch(spec, q, k, positions, top, left, flip, inverse):
     """One launch on ``q`` and ``k`` (either may be None); the results have their layouts."""
     first = q if q is not None else k
-    a = _lib.RotaryParams()
-    a.struct_size = C.sizeof(_lib.RotaryParams)
-    a.dtype = _lib.FEATURE_CODES[first.dtype]
-    a.n, a.tokens, _, a.dim = first.shape
-    a.prefix, a.axes = spec.prefix, len(spec.sections)
-    for i, s in enumerate(spec.sections):
-        a.sections[i] = s
-    a.pairing, a.spectrum, a.inverse, a.base = spec.pairing, spec.spectrum, int(inverse), spec.base
-    if positions is not None:
-        a.position_kind, a.positions = _lib.POSITION_CODES[positions.dtype], positions.data_ptr()
-        st = positions.stride()
-        a.position_strides[:] = st if positions.ndim == 3 else (0,) + st
-    else:
-        a.position_kind = _lib.POS_GRID
-        for i, s in enumerate(spec.grid):
-            a.grid[i] = s
-        a.patch = spec.patch
-        a.top, a.left, a.flip = _address(top), _address(left), _address(flip)
-    outs = []
-    for t, name in ((q, "q"), (k, "k")):
+    n, tokens, _, dim = first.shape
+    ins, outs, heads, addresses, strides = [], [], [], [], []
+    for t in (q, k):
         if t is None:
-            outs.append(None)
+            ins.append(None), outs.append(None), heads.append(0), addresses.append(0), strides.append((_ABSENT, _ABSENT))
             continue
         t = _inner_dense(t)
         out = torch.empty_like(t)
         if out.stride(-1) != 1:                # an expanded input: its copy is laid out by size
             out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        setattr(a, name + "_heads", t.shape[2])
-        setattr(a, name, t.data_ptr())
-        setattr(a, name + "_out", out.data_ptr())
-        getattr(a, name + "_strides")[:] = t.stride()[:3]
-        getattr(a, name + "_out_strides")[:] = out.stride()[:3]
-        outs.append((t, out))
-    _lib.launch_rotary(a, first.device)
-    return tuple(None if o is None else o[1] for o in outs)
+        ins.append(t), outs.append(out), heads.append(t.shape[2]), addresses.append(out.data_ptr())
+        strides.append((t.stride()[:3], out.stride()[:3]))
+    if positions is None:
+        kind, where, step = _lib.POS_GRID, 0, _ABSENT
+    else:
+        kind, where, step = _lib.POSITION_CODES[positions.dtype], positions.data_ptr(), positions.stride()
+        if positions.ndim == 2:
+            step = (0,) + step
+    _lib.launch_rotary((_lib.FEATURE_CODES[first.dtype], n, tokens, spec.prefix, *heads, dim, *spec.head, inverse, kind, spec.middle,
+                        where, *step, *spec.tail, _address(top), _address(left), _address(flip),
+                        _address(ins[0]), _address(ins[1]), *addresses,
+                        *strides[0][0], *strides[1][0], *strides[0][1], *strides[1][1]), first.device)
+    return tuple(outs)
 
 
 class _RotaryEmbedding(torch.autograd.Function):
@@ -333,7 +359,7 @@ class _RotaryEmbedding(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, top, left, flip)
         ctx.spec = spec
-        return _rotary_launch(spec, q, k, positions, top, left, flip, False)
+        return _rotary_launch(spec, q, k, positions, top, left, flip, 0)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -341,7 +367,7 @@ class _RotaryEmbedding(torch.autograd.Function):
         dq = dq if ctx.needs_input_grad[0] else None
         dk = dk if ctx.needs_input_grad[1] else None
         if dq is not None or dk is not None:
-            dq, dk = _rotary_launch(ctx.spec, dq, dk, *ctx.saved_tensors, True)
+            dq, dk = _rotary_launch(ctx.spec, dq, dk, *ctx.saved_tensors, 1)
         return dq, dk, None, None, None, None, None
 
 
@@ -389,24 +415,17 @@ def rotary_embedding(q, k=None, *, sections, positions=None, grid=None, patch: f
         _like(k, q, "k", (n, length, k.shape[2], dim))
         if k.dtype != q.dtype:
             raise TypeError(f"k must be {q.dtype} like q, got {k.dtype}")
-    spec = _Rotary()
-    spec.sections = tuple(int(s) for s in sections)
-    axes = len(spec.sections)
-    if not 1 <= axes <= 3:
-        raise ValueError(f"sections must name one to three axes, got {axes}")
-    if any(s < 0 or s % 2 for s in spec.sections) or sum(spec.sections) > min(dim, 512):
-        raise ValueError(f"sections must be even, not negative, and add up to at most {min(dim, 512)}, got {spec.sections}")
-    spec.base = float(base)
-    if not 0.0 < spec.base < float("inf"):
-        raise ValueError(f"base must be positive, got {base}")
-    spec.pairing = _choice(pairing, _lib.PAIRINGS, "pairing")
-    spec.spectrum = _choice(spectrum, _lib.SPECTRA, "spectrum")
-    spec.prefix = int(prefix)
-    if not 0 <= spec.prefix <= length:
+    if isinstance(grid, int):
+        grid = (grid,)
+    spec = _rotary_spec(tuple(sections), None if grid is None else tuple(grid), patch, base, pairing, spectrum, prefix)
+    axes, prefix = len(spec.sections), spec.prefix
+    if sum(spec.sections) > dim:
+        raise ValueError(f"sections must be even, not negative, and add up to at most {dim}, got {spec.sections}")
+    if not 0 <= prefix <= length:
         raise ValueError(f"prefix must be in [0, {length}], got {prefix}")
     if (positions is None) == (grid is None):
         raise ValueError("exactly one of positions and grid must be given")
-    spec.grid = spec.patch = top_t = left_t = flip_t = None
+    top_t = left_t = flip_t = None
     window = [name for name, v in (("top", top), ("left", left), ("flip_horizontal", flip_horizontal))
               if isinstance(v, torch.Tensor) or v]
     if positions is not None:
@@ -422,14 +441,8 @@ def rotary_embedding(q, k=None, *, sections, positions=None, grid=None, patch: f
         if window or patch != 1:
             raise ValueError(f"{', '.join(window) or 'patch'} belongs to grid, not to positions")
     else:
-        spec.grid = tuple(int(g) for g in ((grid,) if isinstance(grid, int) else grid))
-        if len(spec.grid) != axes or any(g < 0 for g in spec.grid):
-            raise ValueError(f"grid must have {axes} sizes like sections, got {grid}")
-        if torch.Size(spec.grid).numel() != length - spec.prefix:
-            raise ValueError(f"grid {spec.grid} has {torch.Size(spec.grid).numel()} patches for {length - spec.prefix} tokens")
-        spec.patch = float(patch)
-        if not 0.0 < spec.patch < float("inf"):
-            raise ValueError(f"patch must be positive, got {patch}")
+        if math.prod(spec.grid) != length - prefix:
+            raise ValueError(f"grid {spec.grid} has {math.prod(spec.grid)} patches for {length - prefix} tokens")
         if axes < 2 and "top" in window:
             raise ValueError("top needs a height axis")
         _on_cuda(q, "q")
@@ -440,5 +453,5 @@ def rotary_embedding(q, k=None, *, sections, positions=None, grid=None, patch: f
     if _wants_grad(q, k):
         out_q, out_k = _RotaryEmbedding.apply(q, k, positions, top_t, left_t, flip_t, spec)
     else:
-        out_q, out_k = _rotary_launch(spec, q, k, positions, top_t, left_t, flip_t, False)
+        out_q, out_k = _rotary_launch(spec, q, k, positions, top_t, left_t, flip_t, 0)
     return out_q if k is None else (out_q, out_k)

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -86,6 +87,13 @@ class GroupNormParams(C.Structure):
         ("mean", C.c_void_p), ("rstd", C.c_void_p), ("dy", C.c_void_p), ("dx", C.c_void_p),
         ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t),
     ]
+
+
+# The whole of each feature struct in one call (a ctypes field costs as much as all of this); addresses are
+# integers, 0 for NULL.  Native alignment lays the fields out as the C compiler does.
+PACK_GROUP_NORM = struct.Struct("@Iiiiqqiifi11PN")
+PACK_DROPOUT = struct.Struct("@Ii4qIIdQPPPP")
+PACK_ROTARY = struct.Struct("@Iiqq" + "i" * 12 + "dP3q3if" + "P" * 7 + "12q")
 
 
 class DropoutParams(C.Structure):
@@ -177,16 +185,11 @@ def load():
     lib.ta_b200_host_release.restype = C.c_int
     lib.ta_b200_debug_wait.argtypes = [C.c_uint64, C.c_int32]
     lib.ta_b200_debug_wait.restype = C.c_int
-    lib.ta_b200_group_norm.argtypes = [C.POINTER(GroupNormParams), C.c_void_p]
-    lib.ta_b200_group_norm.restype = C.c_int
-    lib.ta_b200_group_norm_backward.argtypes = [C.POINTER(GroupNormParams), C.c_void_p]
-    lib.ta_b200_group_norm_backward.restype = C.c_int
-    lib.ta_b200_group_norm_scratch_bytes.argtypes = [C.POINTER(GroupNormParams), C.c_int32]
+    for fn in (lib.ta_b200_group_norm, lib.ta_b200_group_norm_backward, lib.ta_b200_dropout, lib.ta_b200_rotary):
+        fn.argtypes = [C.c_void_p, C.c_void_p]             # the struct as packed bytes, or a pointer to one
+        fn.restype = C.c_int
+    lib.ta_b200_group_norm_scratch_bytes.argtypes = [C.c_void_p, C.c_int32]
     lib.ta_b200_group_norm_scratch_bytes.restype = C.c_size_t
-    lib.ta_b200_dropout.argtypes = [C.POINTER(DropoutParams), C.c_void_p]
-    lib.ta_b200_dropout.restype = C.c_int
-    lib.ta_b200_rotary.argtypes = [C.POINTER(RotaryParams), C.c_void_p]
-    lib.ta_b200_rotary.restype = C.c_int
     if lib.ta_b200_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libta_b200.so has ABI {lib.ta_b200_abi_version()}, this package expects {ABI_VERSION}")
     _lib = lib
@@ -372,29 +375,39 @@ def store_words(dst: torch.Tensor, a: int, b: int) -> None:
         check(load().ta_b200_store_words(_ptr(dst), int(a) & (2 ** 64 - 1), int(b) & (2 ** 64 - 1), stream), "ta_b200_store_words")
 
 
-def launch_group_norm(params: GroupNormParams, device: torch.device, backward: bool = False) -> None:
-    """Enqueue a group norm (or its backward pass) with the scratch it asks for."""
-    lib = load()
+def _launch_packed(name: str, params: bytes, device: torch.device) -> None:
+    """``name(params, current stream of device)`` with ``device`` current."""
+    fn, idx = getattr(load(), name), device.index
+    if idx == torch.cuda.current_device():
+        rc = fn(params, _stream(device))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(params, _stream(device))
+    if rc:
+        check(rc, name)
+
+
+def launch_group_norm(fields, device: torch.device, backward: bool = False) -> None:
+    """Enqueue a group norm (or its backward pass).  ``fields``: those of ta_b200_group_norm_params after
+    struct_size, without the two of the scratch, which is allocated here as the library asks for it."""
+    size = PACK_GROUP_NORM.size
+    params = PACK_GROUP_NORM.pack(size, *fields, 0, 0)
     with _OnDevice(device):
-        need = int(lib.ta_b200_group_norm_scratch_bytes(C.byref(params), int(backward)))
+        need = load().ta_b200_group_norm_scratch_bytes(params, backward)
         if need:
             scratch = torch.empty(need, dtype=torch.uint8, device=device)      # stream-ordered: may be released after the launch
-            params.scratch, params.scratch_bytes = scratch.data_ptr(), need
-        fn, name = ((lib.ta_b200_group_norm_backward, "ta_b200_group_norm_backward") if backward
-                    else (lib.ta_b200_group_norm, "ta_b200_group_norm"))
-        check(fn(C.byref(params), _stream(device)), name)
+            params = PACK_GROUP_NORM.pack(size, *fields, scratch.data_ptr(), need)
+    _launch_packed("ta_b200_group_norm_backward" if backward else "ta_b200_group_norm", params, device)
 
 
-def launch_dropout(params: DropoutParams, device: torch.device) -> None:
-    lib = load()
-    with _OnDevice(device):
-        check(lib.ta_b200_dropout(C.byref(params), _stream(device)), "ta_b200_dropout")
+def launch_dropout(fields, device: torch.device) -> None:
+    """``fields``: those of ta_b200_dropout_params after struct_size."""
+    _launch_packed("ta_b200_dropout", PACK_DROPOUT.pack(PACK_DROPOUT.size, *fields), device)
 
 
-def launch_rotary(params: RotaryParams, device: torch.device) -> None:
-    lib = load()
-    with _OnDevice(device):
-        check(lib.ta_b200_rotary(C.byref(params), _stream(device)), "ta_b200_rotary")
+def launch_rotary(fields, device: torch.device) -> None:
+    """``fields``: those of ta_b200_rotary_params after struct_size."""
+    _launch_packed("ta_b200_rotary", PACK_ROTARY.pack(PACK_ROTARY.size, *fields), device)
 
 
 def crop_path(path: int) -> None:

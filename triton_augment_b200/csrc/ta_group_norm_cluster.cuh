@@ -6,6 +6,7 @@
 // the first, so a block's whole share is in flight at once and nothing but cp.async.wait_group orders
 // the copies.  The share is loaded in four parts and reduced part by part as they arrive.
 #pragma once
+#include <atomic>
 
 namespace ta {
 
@@ -362,12 +363,20 @@ __host__ inline bool gn_plan(const GnArgs &a, int v, int elem_bytes, bool backwa
     return false;
 }
 
-template <typename Kernel, typename... Args>
-cudaError_t gn_launch_cluster(Kernel kernel, const GnPlan &p, long long samples, cudaStream_t stream, Args... args)
+template <auto kernel, typename... Args>
+cudaError_t gn_launch_cluster( const GnPlan &p, long long samples, cudaStream_t stream, Args... args)
 {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024);
-    if (e == cudaSuccess && p.ranks > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    // once per device: shared memory and cluster size beyond the defaults (setting them twice does no harm)
+    static std::atomic<unsigned> ready{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
+    if (device > 31 || !((ready.load(std::memory_order_acquire) >> device) & 1u)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        if (device <= 31) ready.fetch_or(1u << device, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(samples * p.ranks), p.slabs);
     cfg.blockDim = dim3(p.threads);
@@ -378,20 +387,20 @@ cudaError_t gn_launch_cluster(Kernel kernel, const GnPlan &p, long long samples,
     attr[0].val.clusterDim.x = p.ranks;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = p.ranks > 1 ? 1 : 0;                 // (a cluster of one needs no attribute: 1 us less on the host)
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <typename T> cudaError_t gn_launch_planned(const GnArgs &a, const GnPlan &p, bool backward, cudaStream_t stream)
 {
     if (!backward)
-        return p.threads == 256   ? gn_launch_cluster(gn_cluster_kernel<T, 256, 4>, p, a.n, stream, a, p)
-               : p.threads == 320 ? gn_launch_cluster(gn_cluster_kernel<T, 320, 3>, p, a.n, stream, a, p)
-                                  : gn_launch_cluster(gn_cluster_kernel<T, 512, 2>, p, a.n, stream, a, p);
+        return p.threads == 256   ? gn_launch_cluster<gn_cluster_kernel<T, 256, 4>>(p, a.n, stream, a, p)
+               : p.threads == 320 ? gn_launch_cluster<gn_cluster_kernel<T, 320, 3>>(p, a.n, stream, a, p)
+                                  : gn_launch_cluster<gn_cluster_kernel<T, 512, 2>>(p, a.n, stream, a, p);
     float2 *sums = a.dweight || a.dbias ? a.part : nullptr;
-    const cudaError_t e = p.threads == 192   ? gn_launch_cluster(gn_cluster_grad_kernel<T, 192, 4>, p, a.n, stream, a, p, sums)
-                          : p.threads == 256 ? gn_launch_cluster(gn_cluster_grad_kernel<T, 256, 3>, p, a.n, stream, a, p, sums)
-                                             : gn_launch_cluster(gn_cluster_grad_kernel<T, 384, 2>, p, a.n, stream, a, p, sums);
+    const cudaError_t e = p.threads == 192   ? gn_launch_cluster<gn_cluster_grad_kernel<T, 192, 4>>(p, a.n, stream, a, p, sums)
+                          : p.threads == 256 ? gn_launch_cluster<gn_cluster_grad_kernel<T, 256, 3>>(p, a.n, stream, a, p, sums)
+                                             : gn_launch_cluster<gn_cluster_grad_kernel<T, 384, 2>>(p, a.n, stream, a, p, sums);
     if (e != cudaSuccess || !sums) return e;
     return gn_launch_kernel(gn_grad_params_kernel, dim3((a.channels + 31) / 32), 0, false, stream, a, (const float2 *)sums, a.n);
 }
