@@ -9,7 +9,7 @@ import torch
 import feature_reference as R
 import triton_augment_b200 as ta
 from triton_augment_b200 import _lib
-from triton_augment_b200._functional_features import _mask_layout, _memory_order
+from triton_augment_b200._functional_features import _mask_layout
 
 X = torch.rand(2, 8, 3, 5)
 
@@ -208,33 +208,9 @@ def test_struct_sizes():
     assert [C.sizeof(s) for s in (_lib.GroupNormParams, _lib.DropoutParams, _lib.RotaryParams)] == [144, 96, 280]
 
 
-@pytest.mark.parametrize("struct_type, packer", [(_lib.GroupNormParams, _lib.PACK_GROUP_NORM), (_lib.DropoutParams, _lib.PACK_DROPOUT),
-                                                 (_lib.RotaryParams, _lib.PACK_ROTARY)])
-def test_packed_structs(struct_type, packer):
-    """A struct packed in one call holds every field where the C struct has it."""
-    count = sum(getattr(t, "_length_", 1) for _, t in struct_type._fields_)
-    fields = struct_type.from_buffer_copy(packer.pack(*range(1, count + 1)))
-    got = []
-    for name, t in struct_type._fields_:
-        value = getattr(fields, name)
-        got += list(value) if hasattr(t, "_length_") else [value]
-    assert packer.size == C.sizeof(struct_type) and got == list(range(1, count + 1))
-
-
 # ----------------------------------------------------------------------------- layouts and references
-def test_memory_order():
-    base = torch.rand(2, 3, 4, 5)
-    assert _memory_order(base)[1] is False and _memory_order(base)[0] is base
-    last, is_last = _memory_order(base.permute(0, 3, 1, 2))
-    assert is_last and last.data_ptr() == base.data_ptr() and last.shape == (2, 5, 3, 4)
-    sliced, is_last = _memory_order(base[:, :, :, 1:4])
-    assert not is_last and sliced.is_contiguous() and sliced.shape == (2, 3, 4, 3)
-    clip, is_last = _memory_order(torch.rand(2, 6, 4, 5, 3).permute(0, 1, 4, 2, 3))
-    assert is_last and clip.shape == (2, 6, 3, 4, 5)
-
-
 def test_mask_layout():
-    assert _mask_layout((7, 3), False, 0, False, False) == ((1, 1, 1, 21), 0)
+    assert _mask_layout((2, 5, 3, 4), False, 0, True, False) == ((2, 1, 5, 12), 1)
     assert _mask_layout((2, 5, 3, 4), False, 1, False, False) == ((2, 1, 5, 12), 8)
     assert _mask_layout((2, 5, 3, 4), True, 1, False, False) == ((2, 1, 12, 5), 4)
     assert _mask_layout((2, 5, 3, 4), True, 2, True, False) == ((2, 1, 12, 5), 8 | 1)

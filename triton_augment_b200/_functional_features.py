@@ -26,7 +26,7 @@ __all__ = ["group_norm", "dropout", "rotary_embedding"]
 def _validate_feature_tensor(tensor, name: str) -> None:
     if not isinstance(tensor, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(tensor)}")
-    if tensor.dtype not in _lib.FEATURE_CODES:
+    if tensor.dtype not in _lib.FEATURE_TYPES:
         raise TypeError(f"{name} must be float32, float16 or bfloat16, got {tensor.dtype}")
 
 
@@ -51,67 +51,7 @@ def _choice(value, table, name: str) -> int:
     return code
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _address(t) -> int:
-    return 0 if t is None else t.data_ptr()
-
-
-def _channels_last(t):
-    """``t`` with its channels (dimension -3) last in memory and no gaps; ``t`` itself if it is already."""
-    if t.ndim == 4:
-        return t.contiguous(memory_format=torch.channels_last)
-    last = t.movedim(-3, -1)
-    return t if last.is_contiguous() else last.contiguous().movedim(-1, -3)
-
-
 # ----------------------------------------------------------------------------- group norm
-def _group_norm_fields(x, param, groups, eps, act, samples):
-    """Fields of ta_b200_group_norm_params up to eps (and the padding behind it)."""
-    channels, numel = x.shape[-3], x.numel()
-    return (_lib.FEATURE_CODES[x.dtype], _lib.F32 if param is None else _lib.FEATURE_CODES[param.dtype], act,
-            samples, numel // (samples * channels) if samples else 0, channels, groups, eps, 0)
-
-
-def _group_norm_forward(x, weight, bias, groups, eps, act, samples):
-    """The features with channels last in memory, the result, and the statistics [2, samples * groups]."""
-    x = _channels_last(x)
-    y = torch.empty_like(x)
-    stats = torch.empty(2 * samples * groups, dtype=torch.float32, device=x.device)
-    mean = stats.data_ptr()
-    fields = _group_norm_fields(x, bias if weight is None else weight, groups, eps, act, samples)
-    _lib.launch_group_norm(fields + (x.data_ptr(), _address(weight), _address(bias), y.data_ptr(), mean, mean + 4 * samples * groups,
-                                     0, 0, 0, 0), x.device)
-    return x, y, stats
-
-
-class _GroupNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, samples):
-        x, y, stats = _group_norm_forward(x, weight, bias, groups, eps, act, samples)
-        ctx.save_for_backward(x, weight, bias, stats)
-        ctx.rest = (groups, eps, act, samples)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        groups, eps, act, samples = ctx.rest
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        dy = _channels_last(dy)
-        dx = torch.empty_like(x) if want_x else None
-        dw = torch.empty_like(weight) if want_w else None
-        db = torch.empty_like(bias) if want_b else None
-        mean = stats.data_ptr()
-        fields = _group_norm_fields(x, bias if weight is None else weight, groups, eps, act, samples)
-        _lib.launch_group_norm(fields + (x.data_ptr(), _address(weight), _address(bias), 0, mean, mean + 4 * samples * groups,
-                                         dy.data_ptr(), _address(dx), _address(dw), _address(db)), x.device, backward=True)
-        return dx, dw, db, None, None, None, None
-
-
 def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5, activation: str = "none", *,
                same_on_frame: bool = False) -> torch.Tensor:
     """Group normalisation and an activation in one pass: ``act((x - mean) / sqrt(var + eps) * weight + bias)``.
@@ -145,34 +85,15 @@ def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5, ac
     act = _choice(activation, _lib.ACTIVATIONS, "activation")
     _on_cuda(x, "x")
     samples = 1 if x.ndim == 3 else x.shape[0] * (x.shape[1] if x.ndim == 5 and not same_on_frame else 1)
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    if _wants_grad(x, weight, bias):
-        return _GroupNorm.apply(x, weight, bias, num_groups, float(eps), act, samples)
-    return _group_norm_forward(x, weight, bias, num_groups, float(eps), act, samples)[1]
+    return _lib.torch_binding().group_norm(x, weight, bias, num_groups, float(eps), act, samples)
 
 
 # ----------------------------------------------------------------------------- dropout
 _MODES = {"element": 0, "channel": 1, "pixel": 2, "sample": 3}
 
 
-def _memory_order(x):
-    """``x`` without gaps, row-major or with its channels last, and whether it is the latter."""
-    if x.is_contiguous():
-        return x, False
-    if x.ndim in (3, 4, 5) and x.movedim(-3, -1).is_contiguous():
-        return x, True
-    return x.contiguous(), False
-
-
-def _in_order(t, last):
-    return _channels_last(t) if last else t.contiguous()
-
-
 def _mask_layout(shape, channels_last, mode, same_on_batch, same_on_frame):
     """Four sizes of the tensor in memory order and the bit set of those the mask is shared along."""
-    if mode == 0 and not (same_on_batch or same_on_frame):
-        return (1, 1, 1, math.prod(shape)), 0
     n = shape[0] if len(shape) >= 4 else 1
     t = shape[1] if len(shape) == 5 else 1
     c, plane = shape[-3], shape[-2] * shape[-1]
@@ -180,41 +101,6 @@ def _mask_layout(shape, channels_last, mode, same_on_batch, same_on_frame):
     shared = ((1 if same_on_batch else 0) | (2 if same_on_frame else 0) | (plane_bit if mode in (1, 3) else 0)
               | (chan_bit if mode in (2, 3) else 0))
     return ((n, t, plane, c) if channels_last else (n, t, c, plane)), shared
-
-
-def _dropout_launch(x, residual, layout, p, seed, seed_tensor, offset):
-    y = torch.empty_like(x)
-    sizes, shared = layout
-    _lib.launch_dropout((_lib.FEATURE_CODES[x.dtype], *sizes, shared, offset, p, seed, _address(seed_tensor), x.data_ptr(),
-                         _address(residual), y.data_ptr()), x.device)
-    return y
-
-
-def _dropout_forward(x, residual, p, seed, seed_tensor, offset, mode, same_on_batch, same_on_frame):
-    x, last = _memory_order(x)
-    layout = _mask_layout(x.shape, last, mode, same_on_batch, same_on_frame)
-    if residual is not None:
-        residual = _in_order(residual, last)
-    return _dropout_launch(x, residual, layout, p, seed, seed_tensor, offset), last, layout
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, seed_tensor, offset, mode, same_on_batch, same_on_frame):
-        y, last, layout = _dropout_forward(x, residual, p, seed, seed_tensor, offset, mode, same_on_batch, same_on_frame)
-        ctx.save_for_backward(seed_tensor)
-        ctx.rest = (last, layout, p, seed, offset)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        (seed_tensor,) = ctx.saved_tensors
-        last, layout, p, seed, offset = ctx.rest
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = _dropout_launch(_in_order(dy, last), None, layout, p, seed, seed_tensor, offset)
-        return (dx, dy if ctx.needs_input_grad[1] else None) + (None,) * 7
 
 
 def dropout(x, p: float = 0.5, seed=None, *, offset: int = 0, mode: str = "element", same_on_batch: bool = False,
@@ -268,16 +154,13 @@ def dropout(x, p: float = 0.5, seed=None, *, offset: int = 0, mode: str = "eleme
     if seed is None:
         tensor = torch.randint(-2 ** 63, 2 ** 63 - 1, (1,), dtype=torch.int64, device=x.device)
     same_on_batch, same_on_frame = bool(same_on_batch) and x.ndim >= 4, bool(same_on_frame) and x.ndim == 5
-    args = (p, number, tensor, offset, code, same_on_batch, same_on_frame)
-    if _wants_grad(x, residual):
-        return _Dropout.apply(x, residual, *args)
-    return _dropout_forward(x, residual, *args)[0]
+    return _lib.torch_binding().dropout(x, residual, p, number, tensor, offset, code, same_on_batch, same_on_frame, _mask_layout)
 
 
 # ----------------------------------------------------------------------------- rotary positions
 class _Rotary:
     """What of a call does not depend on its tensors, checked and laid out once per configuration."""
-    __slots__ = ("sections", "grid", "prefix", "head", "middle", "tail")
+    __slots__ = ("sections", "grid", "prefix", "call")
 
     def __init__(self, sections, grid, patch, base, pairing, spectrum, prefix):
         self.sections = tuple(int(s) for s in sections)
@@ -299,11 +182,7 @@ class _Rotary:
                 raise ValueError(f"grid must have {axes} sizes like sections, got {grid}")
             if not 0.0 < patch < float("inf"):
                 raise ValueError(f"patch must be positive, got {patch}")
-        pad = (0,) * (3 - axes)
-        # ta_b200_rotary_params: axes, sections, pairing, spectrum | base | grid, patch
-        self.head = (axes, *self.sections, *pad, pairing, spectrum)
-        self.middle = base
-        self.tail = ((0, 0, 0) if grid is None else self.grid + pad) + (patch,)
+        self.call = _lib.torch_binding().rotary_spec(list(self.sections), pairing, spectrum, self.prefix, base, self.grid, patch)
 
 
 _ROTARY_CACHE = {}
@@ -316,59 +195,6 @@ def _rotary_spec(*key) -> _Rotary:
         if len(_ROTARY_CACHE) < 64:
             _ROTARY_CACHE[key] = spec
     return spec
-
-
-def _inner_dense(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-_ABSENT = (0, 0, 0)
-
-
-def _rotary_launch(spec, q, k, positions, top, left, flip, inverse):
-    """One launch on ``q`` and ``k`` (either may be None); the results have their layouts."""
-    first = q if q is not None else k
-    n, tokens, _, dim = first.shape
-    ins, outs, heads, addresses, strides = [], [], [], [], []
-    for t in (q, k):
-        if t is None:
-            ins.append(None), outs.append(None), heads.append(0), addresses.append(0), strides.append((_ABSENT, _ABSENT))
-            continue
-        t = _inner_dense(t)
-        out = torch.empty_like(t)
-        if out.stride(-1) != 1:                # an expanded input: its copy is laid out by size
-            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        ins.append(t), outs.append(out), heads.append(t.shape[2]), addresses.append(out.data_ptr())
-        strides.append((t.stride()[:3], out.stride()[:3]))
-    if positions is None:
-        kind, where, step = _lib.POS_GRID, 0, _ABSENT
-    else:
-        kind, where, step = _lib.POSITION_CODES[positions.dtype], positions.data_ptr(), positions.stride()
-        if positions.ndim == 2:
-            step = (0,) + step
-    _lib.launch_rotary((_lib.FEATURE_CODES[first.dtype], n, tokens, spec.prefix, *heads, dim, *spec.head, inverse, kind, spec.middle,
-                        where, *step, *spec.tail, _address(top), _address(left), _address(flip),
-                        _address(ins[0]), _address(ins[1]), *addresses,
-                        *strides[0][0], *strides[1][0], *strides[0][1], *strides[1][1]), first.device)
-    return tuple(outs)
-
-
-class _RotaryEmbedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, top, left, flip, spec):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions, top, left, flip)
-        ctx.spec = spec
-        return _rotary_launch(spec, q, k, positions, top, left, flip, 0)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk):
-        dq = dq if ctx.needs_input_grad[0] else None
-        dk = dk if ctx.needs_input_grad[1] else None
-        if dq is not None or dk is not None:
-            dq, dk = _rotary_launch(ctx.spec, dq, dk, *ctx.saved_tensors, 1)
-        return dq, dk, None, None, None, None, None
 
 
 def _per_sample(value, neutral, n, dtype, device, name):
@@ -431,7 +257,7 @@ def rotary_embedding(q, k=None, *, sections, positions=None, grid=None, patch: f
     if positions is not None:
         if not isinstance(positions, torch.Tensor):
             raise TypeError(f"positions must be a torch.Tensor, got {type(positions)}")
-        if positions.dtype not in _lib.POSITION_CODES:
+        if positions.dtype not in _lib.POSITION_TYPES:
             raise TypeError(f"positions must be int64, int32 or float32, got {positions.dtype}")
         if tuple(positions.shape) not in ((length, axes), (n, length, axes)):
             raise ValueError(f"positions must have shape ({length}, {axes}) or ({n}, {length}, {axes}), got {tuple(positions.shape)}")
@@ -450,8 +276,4 @@ def rotary_embedding(q, k=None, *, sections, positions=None, grid=None, patch: f
         left_t = _per_sample(left, 0, n, torch.float32, q.device, "left")
         flip_t = _per_sample(flip_horizontal, False, n, torch.bool, q.device, "flip_horizontal")
     _on_cuda(q, "q")
-    if _wants_grad(q, k):
-        out_q, out_k = _RotaryEmbedding.apply(q, k, positions, top_t, left_t, flip_t, spec)
-    else:
-        out_q, out_k = _rotary_launch(spec, q, k, positions, top_t, left_t, flip_t, 0)
-    return out_q if k is None else (out_q, out_k)
+    return _lib.torch_binding().rotary(q, k, positions, top_t, left_t, flip_t, spec.call)

@@ -7,23 +7,24 @@ and the stream is torch's current stream on the tensor's device.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
-import struct
 
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TA_B200_LIB") or os.path.join(_HERE, "lib", "libta_b200.so")
 
+BINDING_PATH = os.path.join(_HERE, "lib", "_ta_torch.so")
+
 ABI_VERSION = 1
 F32, F16, U8, U8_F16 = 0, 1, 2, 3       # U8 / U8_F16: bytes in (read as value / 255), float32 / float16 out
 BF16 = 4                                # feature operators only, next to F32 and F16
-FEATURE_CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+FEATURE_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 PAIRINGS = {"interleaved": 0, "halves": 1}
 SPECTRA = {"axis": 0, "joint": 1}
-POS_GRID = 0
-POSITION_CODES = {torch.int64: 1, torch.float32: 2, torch.int32: 3}
+POSITION_TYPES = (torch.int64, torch.float32, torch.int32)
 NEAREST, BILINEAR = 0, 1
 CONTRAST_FAST, CONTRAST_MEAN = 0, 1
 ERR_TIMEOUT = -9
@@ -87,13 +88,6 @@ class GroupNormParams(C.Structure):
         ("mean", C.c_void_p), ("rstd", C.c_void_p), ("dy", C.c_void_p), ("dx", C.c_void_p),
         ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t),
     ]
-
-
-# The whole of each feature struct in one call (a ctypes field costs as much as all of this); addresses are
-# integers, 0 for NULL.  Native alignment lays the fields out as the C compiler does.
-PACK_GROUP_NORM = struct.Struct("@Iiiiqqiifi11PN")
-PACK_DROPOUT = struct.Struct("@Ii4qIIdQPPPP")
-PACK_ROTARY = struct.Struct("@Iiqq" + "i" * 12 + "dP3q3if" + "P" * 7 + "12q")
 
 
 class DropoutParams(C.Structure):
@@ -186,7 +180,7 @@ def load():
     lib.ta_b200_debug_wait.argtypes = [C.c_uint64, C.c_int32]
     lib.ta_b200_debug_wait.restype = C.c_int
     for fn in (lib.ta_b200_group_norm, lib.ta_b200_group_norm_backward, lib.ta_b200_dropout, lib.ta_b200_rotary):
-        fn.argtypes = [C.c_void_p, C.c_void_p]             # the struct as packed bytes, or a pointer to one
+        fn.argtypes = [C.c_void_p, C.c_void_p]             # (Python calls go through csrc/ta_torch.cpp; these serve C-level callers)
         fn.restype = C.c_int
     lib.ta_b200_group_norm_scratch_bytes.argtypes = [C.c_void_p, C.c_int32]
     lib.ta_b200_group_norm_scratch_bytes.restype = C.c_size_t
@@ -375,39 +369,23 @@ def store_words(dst: torch.Tensor, a: int, b: int) -> None:
         check(load().ta_b200_store_words(_ptr(dst), int(a) & (2 ** 64 - 1), int(b) & (2 ** 64 - 1), stream), "ta_b200_store_words")
 
 
-def _launch_packed(name: str, params: bytes, device: torch.device) -> None:
-    """``name(params, current stream of device)`` with ``device`` current."""
-    fn, idx = getattr(load(), name), device.index
-    if idx == torch.cuda.current_device():
-        rc = fn(params, _stream(device))
-    else:
-        with torch.cuda.device(idx):
-            rc = fn(params, _stream(device))
-    if rc:
-        check(rc, name)
+_binding = None
 
 
-def launch_group_norm(fields, device: torch.device, backward: bool = False) -> None:
-    """Enqueue a group norm (or its backward pass).  ``fields``: those of ta_b200_group_norm_params after
-    struct_size, without the two of the scratch, which is allocated here as the library asks for it."""
-    size = PACK_GROUP_NORM.size
-    params = PACK_GROUP_NORM.pack(size, *fields, 0, 0)
-    with _OnDevice(device):
-        need = load().ta_b200_group_norm_scratch_bytes(params, backward)
-        if need:
-            scratch = torch.empty(need, dtype=torch.uint8, device=device)      # stream-ordered: may be released after the launch
-            params = PACK_GROUP_NORM.pack(size, *fields, scratch.data_ptr(), need)
-    _launch_packed("ta_b200_group_norm_backward" if backward else "ta_b200_group_norm", params, device)
-
-
-def launch_dropout(fields, device: torch.device) -> None:
-    """``fields``: those of ta_b200_dropout_params after struct_size."""
-    _launch_packed("ta_b200_dropout", PACK_DROPOUT.pack(PACK_DROPOUT.size, *fields), device)
-
-
-def launch_rotary(fields, device: torch.device) -> None:
-    """``fields``: those of ta_b200_rotary_params after struct_size."""
-    _launch_packed("ta_b200_rotary", PACK_ROTARY.pack(PACK_ROTARY.size, *fields), device)
+def torch_binding():
+    """The feature operators as torch functions (csrc/ta_torch.cpp), bound to the loaded library (once).
+    Raises if it has not been built."""
+    global _binding
+    if _binding is None:
+        load()
+        if not os.path.exists(BINDING_PATH):
+            raise RuntimeError(f"{BINDING_PATH} is missing: build it with `python -m triton_augment_b200.build`")
+        spec = importlib.util.spec_from_file_location("_ta_torch", BINDING_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(LIB_PATH, LibraryError)
+        _binding = module
+    return _binding
 
 
 def crop_path(path: int) -> None:

@@ -22,8 +22,8 @@ static int group_norm_args(const ta_b200_group_norm_params *p, bool backward, Gn
         return fail(TA_B200_ERR_SHAPE, "bad sizes n=%lld rows=%lld channels=%d groups=%d (channels must be a multiple of groups)",
                     (long long)p->n, (long long)p->rows, p->channels, p->groups);
     if (!(p->eps >= 0.0f)) return fail(TA_B200_ERR_SHAPE, "eps must not be negative");
-    if (p->n >= (1 << 22) || p->rows >= (1LL << 31) || p->channels > (1 << 22) || (double)p->n * p->rows * p->channels >= 1.0e15)
-        return fail(TA_B200_ERR_TOO_LARGE, "at most 2^22 samples, 2^31 rows and 2^22 channels per call");
+    if (p->n >= (1 << 22) || p->rows >= (1LL << 31) || p->channels > (1 << 20) || (double)p->n * p->rows * p->channels >= 1.0e15)
+        return fail(TA_B200_ERR_TOO_LARGE, "at most 2^22 samples, 2^31 rows and 2^20 channels per call");
     const bool empty = p->n == 0 || p->rows == 0;
     if (!empty && (!p->x || (backward ? !p->dy || !p->mean || !p->rstd : !p->y || !p->mean || !p->rstd)))
         return fail(TA_B200_ERR_NULL, "x, mean, rstd and y (forward) or dy (backward) are required");
@@ -37,6 +37,12 @@ static int group_norm_args(const ta_b200_group_norm_params *p, bool backward, Gn
     a.param_code = p->param_dtype; a.act = p->activation; a.eps = p->eps;
     a.wide_params = p->param_dtype == TA_B200_F32 && (((uintptr_t)p->weight | (uintptr_t)p->bias) % 16) == 0;
     return TA_B200_OK;
+}
+
+static size_t group_norm_scratch(int dtype, const GnArgs &a, bool backward)
+{
+    return dtype == TA_B200_F32 ? scratch_group_norm_f32(a, backward) : dtype == TA_B200_F16 ? scratch_group_norm_f16(a, backward)
+                                                                                           : scratch_group_norm_bf16(a, backward);
 }
 
 static int group_norm(const ta_b200_group_norm_params *p, bool backward, cudaStream_t stream)
@@ -60,7 +66,7 @@ static int group_norm(const ta_b200_group_norm_params *p, bool backward, cudaStr
     rc = current_device(&s, nullptr);
     if (rc != TA_B200_OK) return rc;
     a.sm_count = s->sm_count;
-    const size_t need = group_norm_scratch_bytes(a, (int)es, backward);
+    const size_t need = group_norm_scratch(p->dtype, a, backward);
     if (need > 0 && (!p->scratch || p->scratch_bytes < need || (uintptr_t)p->scratch % 16))
         return fail(TA_B200_ERR_SCRATCH, "scratch must be 16-byte aligned and hold %zu bytes", need);
     cudaError_t e = p->dtype == TA_B200_F32 ? launch_group_norm_f32(a, backward, stream)
@@ -227,7 +233,7 @@ size_t ta_b200_group_norm_scratch_bytes(const ta_b200_group_norm_params *p, int3
     ta::DeviceState *s = nullptr;
     if (ta::current_device(&s, nullptr) != TA_B200_OK) return 0;
     a.sm_count = s->sm_count;
-    return ta::group_norm_scratch_bytes(a, ta::feature_bytes(p->dtype), backward != 0);
+    return ta::group_norm_scratch(p->dtype, a, backward != 0);
 }
 
 int ta_b200_dropout(const ta_b200_dropout_params *p, void *stream) { return ta::dropout(p, (cudaStream_t)stream); }

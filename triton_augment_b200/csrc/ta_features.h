@@ -13,7 +13,7 @@ struct GnArgs {
     const void *x, *weight, *bias, *dy;
     void *y, *dx, *dweight, *dbias;
     float *mean, *rstd;             // [n, groups]
-    float2 *part, *channel_part;    // scratch, see group_norm_scratch_bytes()
+    float2 *part, *channel_part;    // scratch, see scratch_group_norm_*()
     long long n, rows;
     int channels, groups, cpg;      // cpg = channels / groups
     int param_code, act;
@@ -23,7 +23,9 @@ struct GnArgs {
 };
 
 // scratch of a forward (backward = false) or backward call, bytes
-size_t group_norm_scratch_bytes(const GnArgs &a, int elem_bytes, bool backward);
+size_t scratch_group_norm_f32(const GnArgs &a, bool backward);
+size_t scratch_group_norm_f16(const GnArgs &a, bool backward);
+size_t scratch_group_norm_bf16(const GnArgs &a, bool backward);
 cudaError_t launch_group_norm_f32(const GnArgs &a, bool backward, cudaStream_t stream);
 cudaError_t launch_group_norm_f16(const GnArgs &a, bool backward, cudaStream_t stream);
 cudaError_t launch_group_norm_bf16(const GnArgs &a, bool backward, cudaStream_t stream);

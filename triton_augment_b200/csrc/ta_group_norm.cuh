@@ -141,18 +141,18 @@ template <int V, typename Get> __device__ __forceinline__ void spread_groups(int
 
 __device__ __forceinline__ float half_of_pair(float2 v, int j) { return j % 2 ? v.y : v.x; }
 
-// Values of V channels added up over neighbours of one group, `fold` at a time, into dst[]
-template <int V> __device__ __forceinline__ void store_folded(float *dst, float (&s)[V], int fold)
+// Pairs of values of V channels added up over neighbours of one group, `fold` at a time, into dst[]
+template <int V> __device__ __forceinline__ void store_folded(float2 *dst, const float2 (&a)[(V + 1) / 2], const float2 (&b)[(V + 1) / 2], int fold)
 {
-    if constexpr (V >= 2) if (fold >= 2) {
+    float2 s[V];
 #pragma unroll
-        for (int i = 0; i < V; i += 2) s[i] += s[i + 1];
-    }
-    if constexpr (V >= 4) if (fold >= 4) {
+    for (int i = 0; i < V; ++i) s[i] = make_float2(half_of_pair(a[i / 2], i), half_of_pair(b[i / 2], i));
 #pragma unroll
-        for (int i = 0; i < V; i += 4) s[i] += s[i + 2];
-    }
-    if constexpr (V >= 8) if (fold >= 8) s[0] += s[4];
+    for (int w = 1; w < V; w *= 2)
+        if (w < fold) {
+#pragma unroll
+            for (int i = 0; i < V; i += 2 * w) s[i] = add2(s[i], s[i + w]);
+        }
     if (fold == V) { dst[0] = s[0]; return; }
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -163,6 +163,7 @@ template <int V> __device__ __forceinline__ void store_folded(float *dst, float 
 // `width` neighbouring values in each of a number of rows.
 struct GnLanes {
     int lanes, width, row_step, entry_step;              // a lane's next entry: row_step rows and entry_step values on
+    FastDiv width_div;
 };
 __host__ inline GnLanes gn_lanes(int groups, int threads, int width)
 {
@@ -172,7 +173,18 @@ __host__ inline GnLanes gn_lanes(int groups, int threads, int width)
     l.width = width;
     l.row_step = l.lanes / width;
     l.entry_step = l.lanes % width;
+    l.width_div = fast_div_of(width);
     return l;
+}
+__device__ __forceinline__ float2 lane_sum(float2 v, int lanes)
+{
+    const auto add = [&](int o) { v = add2(v, make_float2(__shfl_down_sync(0xffffffffu, v.x, o), __shfl_down_sync(0xffffffffu, v.y, o))); };
+    if (lanes > 16) add(16);
+    if (lanes > 8) add(8);
+    if (lanes > 4) add(4);
+    if (lanes > 2) add(2);
+    if (lanes > 1) add(1);
+    return v;
 }
 __device__ __forceinline__ float lane_sum(float v, int lanes)
 {
@@ -180,14 +192,14 @@ __device__ __forceinline__ float lane_sum(float v, int lanes)
     return v;
 }
 // Sum of a group's entries in its lane 0 (all threads of the block call it together)
-__device__ __forceinline__ float group_sum(const GnLanes &l, const float *red, int stride, int rows, int width, int g, bool valid)
+__device__ __forceinline__ float2 group_sum(const GnLanes &l, const float2 *red, int stride, int rows, int width, int g, bool valid)
 {
-    float s = 0.0f;
+    float2 s = make_float2(0.0f, 0.0f);
     if (valid) {
         const int lane = threadIdx.x & (l.lanes - 1);
-        int r = lane / l.width, e = lane - r * l.width;
+        int r = (int)fast_div(lane, l.width_div), e = lane - r * l.width;
         while (r < rows) {
-            if (e < width) s += red[r * stride + g * l.width + e];
+            if (e < width) s = add2(s, red[r * stride + g * l.width + e]);
             r += l.row_step;
             e += l.entry_step;
             if (e >= l.width) { e -= l.width; ++r; }
@@ -241,7 +253,7 @@ __host__ inline GnShape gn_shape(const GnArgs &a, int v, bool backward)
     s.rows_per_step = kGnThreads / s.tile;
     s.fold = v;
     while (a.cpg % s.fold) s.fold /= 2;
-    s.columns = gn_lanes(s.groups_per_tile, kGnThreads, backward ? (s.split == 1 ? a.cpg : s.tile * v) : (s.split == 1 ? a.cpg : s.tile * v) / s.fold);
+    s.columns = gn_lanes(s.groups_per_tile, kGnThreads, (s.split == 1 ? a.cpg : s.tile * v) / s.fold);
     s.finish_lanes = s.columns.lanes;
     // one wave of blocks where the samples allow it, at least four steps a thread
     const long long want = (long long)(backward ? kGnBlocksBackward : kGnBlocksForward) * a.sm_count / (a.n * s.tiles);
@@ -282,6 +294,20 @@ struct GnPlace {
     __device__ __forceinline__ int count(const GnShape &s) const { return active && rows > r ? (rows - r + s.rows_per_step - 1) / s.rows_per_step : 0; }
 };
 
+// The cluster's barrier in two halves: every thread of every block arrives once and waits once per phase.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// *ptr of the block with cluster rank `rank`
+__device__ __forceinline__ float2 load_rank(const float2 *ptr, int rank)
+{
+    uint32_t remote;
+    float2 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(ptr)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote) : "memory");
+    return v;
+}
+
 // The second launch of a pass may start while the first one ends (programmatic dependent launch): what
 // does not depend on the first is fetched before gn_wait_first().
 __device__ __forceinline__ void gn_allow_second() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -290,7 +316,7 @@ __device__ __forceinline__ void gn_wait_first() { asm volatile("griddepcontrol.w
 constexpr int kGnUnroll = 4;            // rows a thread has in flight
 
 // ----------------------------------------------------------------------------- forward
-// Sums of differences to a thread's pivot (its first value, negated in pv) and of their squares, per channel
+// Sums of differences to the group's pivot (negated in pv) and of their squares, per channel
 template <int P, typename Vec> __device__ __forceinline__ void add_moments(const Vec &p, const float2 (&pv)[P], float2 (&sm)[P], float2 (&s2)[P])
 {
     float2 f[P];
@@ -302,26 +328,24 @@ template <int P, typename Vec> __device__ __forceinline__ void add_moments(const
         s2[j] = fma2(d, d, s2[j]);
     }
 }
-// Per channel, the squared deviations of the thread's values from its group's mean: those from the
-// thread's mean, max(s2 - sm^2 / count, 0), and count times the square of the distance of the two means
-template <int V> __device__ __forceinline__ void deviations(int group, int left, int cpg, int count, const float2 (&pv)[(V + 1) / 2],
-                                                            const float2 (&sm)[(V + 1) / 2], const float2 (&s2)[(V + 1) / 2], const float *means, float (&out)[V])
+// (mean, sum of squared deviations) from the pivot and the sums of differences to it and of their squares
+__device__ __forceinline__ float2 moments_of(float pivot, float2 t, float inv)
 {
-    constexpr int P = (V + 1) / 2;
-    float2 m[P], unused[P];
-    spread_groups<V>(group, left, cpg, [&](int g) { return make_float2(means[g], 0.0f); }, m, unused);
-    const float n = (float)count, inv = count > 0 ? 1.0f / n : 0.0f;
+    const float q = fmaf(-t.x * inv, t.x, t.y);
+    return make_float2(fmaf(t.x, inv, pivot), q < 0.0f ? 0.0f : q);       // (a NaN stays)
+}
+template <int P, typename Vec> __device__ __forceinline__ void add_values(const Vec &p, float2 (&sm)[P])
+{
+    float2 f[P];
+    p.unpack(f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float s = half_of_pair(sm[j / 2], j), q = half_of_pair(s2[j / 2], j);
-        const float own = fmaf(-s * inv, s, q), d = fmaf(s, inv, -half_of_pair(pv[j / 2], j)) - half_of_pair(m[j / 2], j);
-        out[j] = fmaf(n * d, d, own < 0.0f ? 0.0f : own);          // (a NaN stays)
-    }
+    for (int j = 0; j < P; ++j) sm[j] = add2(sm[j], f[j]);
 }
 
-// Per (sample, group, chunk): mean and sum of squared deviations from it.  A thread sums differences to the
-// first value it sees, so that a mean far from zero cancels nothing; the block adds up its means first and
-// then the deviations from the result, and so do the chunks.
+// Per (sample, group, chunk): mean and sum of squared deviations from it.  The block takes the mean of its first
+// rows as pivot and sums differences to it and their squares.  The share of the pivot's rows is at
+// least 1 / 512 of the block's, so its distance to the block's mean is at most 23 spreads, and as a rule far below one:
+// the difference of sums at the end loses next to nothing however far from zero the values lie.
 template <typename T, int V>
 __global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_stats_kernel(const GnArgs a, const GnShape s)
 {
@@ -329,56 +353,61 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_stats_kernel(
     const GnPlace at(a, s, blockIdx.x);
     const int count = at.count(s);
     constexpr int P = Pack<T, V>::P;
+    __shared__ float2 red[kGnThreads * V];                // [row slot][folded channel]
+    __shared__ float pivot[kGnThreads * V];               // [group]
+    const int per_vec = V / s.fold, stride = s.tile * per_vec, groups = at.groups(a, s);
+    const int width = s.split == 1 ? s.columns.width : at.width(s) * per_vec;
+    float2 *slot = red + at.r * stride + at.v * per_vec;
+    const bool holds = at.r < s.rows_per_step;
+    const int per_pass = kGnThreads / s.columns.lanes, lane = threadIdx.x & (s.columns.lanes - 1), mine = threadIdx.x / (unsigned)s.columns.lanes;
+    const T *ptr = (const T *)a.x + (at.n * a.rows + at.row0 + at.r) * a.channels + at.vec * V;
+    const long long step = (long long)s.rows_per_step * a.channels;
     float2 pv[P], sm[P], s2[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) pv[j] = sm[j] = s2[j] = both(0.0f);
-    if (count > 0) {
-        const T *ptr = (const T *)a.x + (at.n * a.rows + at.row0 + at.r) * a.channels + at.vec * V;
-        const long long step = (long long)s.rows_per_step * a.channels;
-        Pack<T, V> p[kGnUnroll];
-        p[0].load(ptr);
-        p[0].unpack(pv);
+    Pack<T, V> p[kGnUnroll];
 #pragma unroll
-        for (int j = 0; j < P; ++j) pv[j] = neg2(pv[j]);
-        int i = 0;
-        for (; i + kGnUnroll <= count; i += kGnUnroll, ptr += kGnUnroll * step) {
+    for (int u = 0; u < kGnUnroll; ++u)
+        if (u < count) p[u].load(ptr + u * step);
 #pragma unroll
-            for (int u = 0; u < kGnUnroll; ++u) p[u].load(ptr + u * step);
-#pragma unroll
-            for (int u = 0; u < kGnUnroll; ++u) add_moments<P>(p[u], pv, sm, s2);
-        }
-        for (; i < count; ++i, ptr += step) {
-            p[0].load(ptr);
-            add_moments<P>(p[0], pv, sm, s2);
-        }
+    for (int u = 0; u < kGnUnroll; ++u)
+        if (u < count) add_values<P>(p[u], sm);
+    if (holds) store_folded<V>(slot, sm, s2, s.fold);
+    __syncthreads();
+    const float first_inv = 1.0f / ((float)min(at.rows, kGnUnroll * s.rows_per_step) * (float)(width * s.fold));
+    for (int base = 0; base < groups; base += per_pass) {
+        const int g = base + mine;
+        const float2 t = group_sum(s.columns, red, stride, s.rows_per_step, width, g, g < groups);
+        if (g < groups && lane == 0) pivot[g] = t.x * first_inv;
     }
-    __shared__ float red[kGnThreads * V], block_mean[kGnThreads * V];       // [row slot][folded channel], [group]
-    const int per_vec = V / s.fold, stride = s.tile * per_vec, groups = at.groups(a, s);
-    const int width = s.split == 1 ? s.columns.width : at.width(s) * per_vec;
-    float *slot = red + at.r * stride + at.v * per_vec;
-    const bool holds = at.r < s.rows_per_step;
-    float t[V];
+    __syncthreads();
+    const int group = at.active ? (at.vec * V) / a.cpg - at.group0 : 0;
+    spread_groups<V>(group, at.active ? a.cpg - (at.vec * V) % a.cpg : V, a.cpg, [&](int g) { return make_float2(-pivot[g], 0.0f); }, pv, sm);
 #pragma unroll
-    for (int j = 0; j < V; ++j) t[j] = fmaf((float)-count, half_of_pair(pv[j / 2], j), half_of_pair(sm[j / 2], j));        // the plain sum
-    if (holds) store_folded<V>(slot, t, s.fold);
+    for (int u = 0; u < kGnUnroll; ++u)
+        if (u < count) add_moments<P>(p[u], pv, sm, s2);
+    int i = kGnUnroll;
+    ptr += kGnUnroll * step;
+    for (; i + kGnUnroll <= count; i += kGnUnroll, ptr += kGnUnroll * step) {
+#pragma unroll
+        for (int u = 0; u < kGnUnroll; ++u) p[u].load(ptr + u * step);
+#pragma unroll
+        for (int u = 0; u < kGnUnroll; ++u) add_moments<P>(p[u], pv, sm, s2);
+    }
+#pragma unroll
+    for (int u = 0; u < kGnUnroll - 1; ++u)
+        if (i + u < count) p[u].load(ptr + u * step);
+#pragma unroll
+    for (int u = 0; u < kGnUnroll - 1; ++u)
+        if (i + u < count) add_moments<P>(p[u], pv, sm, s2);
+    if (holds) store_folded<V>(slot, sm, s2, s.fold);
     __syncthreads();
     const float inv = 1.0f / ((float)at.rows * (float)(width * s.fold));
-    const int per_pass = kGnThreads / s.columns.lanes, lane = threadIdx.x & (s.columns.lanes - 1), mine = threadIdx.x / s.columns.lanes;
     for (int base = 0; base < groups; base += per_pass) {
         const int g = base + mine;
-        const float m = group_sum(s.columns, red, stride, s.rows_per_step, width, g, g < groups) * inv;
-        if (g < groups && lane == 0) block_mean[g] = m;
-    }
-    __syncthreads();
-    // deviations from the block's mean: those from the thread's own mean, and that mean's
-    deviations<V>(at.active ? (at.vec * V) / a.cpg - at.group0 : 0, at.active ? a.cpg - (at.vec * V) % a.cpg : V, a.cpg, count, pv, sm, s2, block_mean, t);
-    if (holds) store_folded<V>(slot, t, s.fold);
-    __syncthreads();
-    for (int base = 0; base < groups; base += per_pass) {
-        const int g = base + mine;
-        const float q = group_sum(s.columns, red, stride, s.rows_per_step, width, g, g < groups);
+        const float2 t = group_sum(s.columns, red, stride, s.rows_per_step, width, g, g < groups);
         if (g < groups && lane == 0)
-            a.part[(((long long)at.n * a.groups + at.group0 + g) * s.chunks + at.chunk) * s.split + at.piece] = make_float2(block_mean[g], q);
+            a.part[(((long long)at.n * a.groups + at.group0 + g) * s.chunks + at.chunk) * s.split + at.piece] = moments_of(pivot[g], t, inv);
     }
 }
 
@@ -508,7 +537,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_sums_ke
     const GnPlace at(a, s, blockIdx.x);
     const int count = at.count(s), c0 = at.vec * V;
     constexpr int P = Pack<T, V>::P, U = kGnUnroll / 2;
-    __shared__ float2 acc[kGnThreads * V];                // [row slot][channel of the tile], then slot 0 the sums
+    __shared__ float2 acc[kGnThreads * V];                // [row slot][folded channel], then [row slot][channel]
     {
         const long long g0 = (long long)at.n * a.groups;
         float2 mean[P], scale[P], bias[P], rstd[P], sgx[P], sg[P];
@@ -545,70 +574,75 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_sums_ke
                 add(x[0], d[0]);
             }
         });
+        // sums of (u xhat, rstd u) of the groups: u xhat = g scale (x - mean)
+        const int per_vec = V / s.fold, stride = s.tile * per_vec, groups = at.groups(a, s), lanes = s.columns.lanes, lane = threadIdx.x & (lanes - 1);
+        const int width = s.split == 1 ? s.columns.width : at.width(s) * per_vec;
+        if (at.r < s.rows_per_step) {
+            float2 ux[P], u[P];
+#pragma unroll
+            for (int j = 0; j < P; ++j) { ux[j] = mul2(scale[j], sgx[j]); u[j] = mul2(scale[j], sg[j]); }
+            store_folded<V>(acc + at.r * stride + at.v * per_vec, ux, u, s.fold);
+        }
+        __syncthreads();
+        for (int base = 0; base < groups; base += kGnThreads / lanes) {
+            const int g = base + threadIdx.x / (unsigned)lanes;
+            const float2 t = group_sum(s.columns, acc, stride, s.rows_per_step, width, g, g < groups);
+            if (g < groups && lane == 0)
+                a.part[(((long long)at.n * a.groups + at.group0 + g) * s.chunks + at.chunk) * s.split + at.piece] = t;
+        }
+        if (!a.dweight && !a.dbias) return;
+        __syncthreads();
         if (at.r < s.rows_per_step) {
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                acc[(at.r * s.tile + at.v) * V + j] = j % 2 ? make_float2(sgx[j / 2].y * rstd[j / 2].y, sg[j / 2].y)
-                                                            : make_float2(sgx[j / 2].x * rstd[j / 2].x, sg[j / 2].x);
+            for (int j = 0; j < P; ++j) {
+                const float2 gx = mul2(sgx[j], rstd[j]);
+                float2 *to = acc + (at.r * s.tile + at.v) * V + 2 * j;
+                to[0] = make_float2(gx.x, sg[j].x);
+                if (V > 1) to[V > 1 ? 1 : 0] = make_float2(gx.y, sg[j].y);
+            }
         }
     }
     __syncthreads();
     const int tile_c0 = (at.vec - at.v) * V, channels = at.width(s) * V;
     float2 *chan = a.channel_part + (long long)at.item * a.channels + tile_c0;
     sum_columns(acc, s.tile * V, channels, s.rows_per_step, kGnThreads);
-    if (a.dweight || a.dbias)
-        for (int c = threadIdx.x; c < channels; c += kGnThreads) chan[c] = acc[c];
-    const int groups = at.groups(a, s), lanes = s.columns.lanes, lane = threadIdx.x & (lanes - 1), width = s.split == 1 ? a.cpg : channels;
-    for (int base = 0; base < groups; base += kGnThreads / lanes) {
-        const int g = base + threadIdx.x / lanes;
-        float ux = 0.0f, u = 0.0f;
-        if (g < groups)
-            for (int e = lane; e < width; e += lanes) {
-                const int c = g * width + e;
-                const float w = a.weight ? load_code(a.weight, a.param_code, tile_c0 + c) : 1.0f;
-                ux = fmaf(w, acc[c].x, ux);
-                u = fmaf(w, acc[c].y, u);
-            }
-        ux = lane_sum(ux, lanes);
-        u = lane_sum(u, lanes);
-        if (g < groups && lane == 0)
-            a.part[(((long long)at.n * a.groups + at.group0 + g) * s.chunks + at.chunk) * s.split + at.piece] = make_float2(ux, u);
-    }
+    for (int c = threadIdx.x; c < channels; c += kGnThreads) chan[c] = acc[c];
 }
 
-// dweight and dbias of 32 channels: the channel sums of all samples and chunks, always added in the same order
-__device__ __forceinline__ void gn_param_grads(const GnArgs &a, const float2 *sums, long long rows, int block, float2 (*acc)[33])
-{
-    const int x = threadIdx.x % 32, y = threadIdx.x / 32, lanes = kGnThreads / 32, c = block * 32 + x;
-    float gx = 0.0f, g = 0.0f;
-    if (c < a.channels) {
-#pragma unroll 8
-        for (long long i = y; i < rows; i += lanes) {
-            const float2 p = sums[i * a.channels + c];
-            gx += p.x; g += p.y;
-        }
-    }
-    acc[y][x] = make_float2(gx, g);
-    __syncthreads();
-    if (y == 0 && c < a.channels) {
-        gx = g = 0.0f;
-        for (int j = 0; j < lanes; ++j) { gx += acc[j][x].x; g += acc[j][x].y; }
-        if (a.dweight) store_code(a.dweight, a.param_code, c, gx);
-        if (a.dbias) store_code(a.dbias, a.param_code, c, g);
-    }
-}
-
+// dweight and dbias of 32 channels by a cluster: the channel sums of all samples and chunks, a share of the rows to
+// each block, always added in the same order
+constexpr int kGnParamRanks = 8;
 static __global__ void __launch_bounds__(kGnThreads) gn_grad_params_kernel(const GnArgs a, const float2 *sums, const long long rows)
 {
-    __shared__ float2 acc[kGnThreads / 32][33];
-    gn_wait_first();
-    gn_param_grads(a, sums, rows, blockIdx.x, acc);
+    __shared__ float2 acc[kGnThreads / 32][33], share[32];
+    const int x = threadIdx.x % 32, y = threadIdx.x / 32, lanes = kGnThreads / 32, c = blockIdx.y * 32 + x;
+    const int ranks = gridDim.x, rank = blockIdx.x;
+    float2 t = make_float2(0.0f, 0.0f);
+    if (c < a.channels) {
+#pragma unroll 8
+        for (long long i = rank * lanes + y; i < rows; i += lanes * ranks) t = add2(t, sums[i * a.channels + c]);
+    }
+    acc[y][x] = t;
+    __syncthreads();
+    if (y == 0) {
+        t = acc[0][x];
+        for (int j = 1; j < lanes; ++j) t = add2(t, acc[j][x]);
+        share[x] = t;
+    }
+    if (ranks > 1) { cluster_arrive(); cluster_wait(); }
+    else __syncthreads();
+    if (rank == 0 && y == 0 && c < a.channels) {
+        for (int k = 1; k < ranks; ++k) t = add2(t, load_rank(share + x, k));
+        if (a.dweight) store_code(a.dweight, a.param_code, c, t.x);
+        if (a.dbias) store_code(a.dbias, a.param_code, c, t.y);
+    }
+    if (ranks > 1) { cluster_arrive(); cluster_wait(); }
 }
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_input_kernel(const GnArgs a, const GnShape s)
 {
-    extern __shared__ float2 stat[];                      // [groups_per_tile] means of (u xhat, u)
+    extern __shared__ float2 stat[];                      // [groups_per_tile] means of (u xhat, rstd u)
     const GnPlace at(a, s, gridDim.x - 1 - blockIdx.x);
     const int count = at.count(s), c0 = at.vec * V;
     constexpr int P = Pack<T, V>::P, U = kGnUnroll / 2;
@@ -638,10 +672,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_input_k
     __syncthreads();
     spread_groups<V>(group - at.group0, left, a.cpg, [&](int g) { return make_float2(-stat[g].x, -stat[g].y); }, m_ux, m_u);
 #pragma unroll
-    for (int j = 0; j < P; ++j) {                         // dx = g scale - ((x - mean) m_ux + m_u)
-        m_ux[j] = mul2(m_ux[j], mul2(rstd[j], rstd[j]));
-        m_u[j] = mul2(m_u[j], rstd[j]);
-    }
+    for (int j = 0; j < P; ++j) m_ux[j] = mul2(m_ux[j], mul2(rstd[j], rstd[j]));       // dx = g scale - ((x - mean) m_ux + m_u)
     const long long first = (at.n * a.rows + at.row0 + at.r) * a.channels + c0, step = (long long)s.rows_per_step * a.channels;
     const T *px = (const T *)a.x + first, *pd = (const T *)a.dy + first;
     T *out = (T *)a.dx + first;
@@ -691,6 +722,22 @@ cudaError_t gn_launch_kernel(Kernel kernel, dim3 grid, size_t smem, bool depende
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+inline cudaError_t gn_launch_params(const GnArgs &a, const float2 *sums, long long rows, cudaStream_t stream)
+{
+    cudaLaunchConfig_t cfg = {};
+    const int ranks = rows >= 64 ? kGnParamRanks : 1;    // (fewer rows are one block's work)
+    cfg.gridDim = dim3(ranks, (a.channels + 31) / 32);
+    cfg.blockDim = dim3(kGnThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ranks > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, gn_grad_params_kernel, a, sums, rows);
+}
+
 template <typename T, int V> cudaError_t gn_launch_streaming(const GnArgs &all, bool backward, cudaStream_t stream)
 {
     GnArgs a = all;
@@ -706,7 +753,7 @@ template <typename T, int V> cudaError_t gn_launch_streaming(const GnArgs &all, 
     e = gn_launch_kernel(gn_grad_sums_kernel<T, V>, grid, 0, false, stream, a, s);
     if (e == cudaSuccess && a.dx) e = gn_launch_kernel(gn_grad_input_kernel<T, V>, grid, smem, true, stream, a, s);
     if (e == cudaSuccess && (a.dweight || a.dbias))
-        e = gn_launch_kernel(gn_grad_params_kernel, dim3((a.channels + 31) / 32), 0, false, stream, a, (const float2 *)a.channel_part, a.n * s.chunks);
+        e = gn_launch_params(a, a.channel_part, a.n * s.chunks, stream);
     return e;
 }
 
@@ -730,13 +777,24 @@ template <typename T> cudaError_t gn_launch(const GnArgs &a, bool backward, cuda
 {
     const int v = gn_vector(a, sizeof(T));
     GnPlan plan;
-    if (gn_plan(a, v, sizeof(T), backward, plan)) return gn_launch_planned<T>(a, plan, backward, stream);
+    if (gn_plan<T>(a, v, backward, plan)) return gn_launch_planned<T>(a, plan, backward, stream);
     switch (v) {
     case 8: if constexpr (sizeof(T) == 2) return gn_launch_streaming<T, 8>(a, backward, stream);
     case 4: return gn_launch_streaming<T, 4>(a, backward, stream);
     case 2: return gn_launch_streaming<T, 2>(a, backward, stream);
     default: return gn_launch_streaming<T, 1>(a, backward, stream);
     }
+}
+
+// scratch of a call, bytes
+template <typename T> size_t gn_scratch_bytes(const GnArgs &a, bool backward)
+{
+    const int v = gn_vector(a, sizeof(T));
+    const bool params = backward && (a.dweight || a.dbias);
+    GnPlan plan;
+    if (gn_plan<T>(a, v, backward, plan)) return params ? (size_t)a.n * plan.ranks * a.channels * sizeof(float2) : 0;
+    const GnShape s = gn_shape(a, v, backward);
+    return ((size_t)a.n * a.groups * s.chunks * s.split + (params ? (size_t)a.n * s.chunks * a.channels : 0)) * sizeof(float2);
 }
 
 }  // namespace ta
