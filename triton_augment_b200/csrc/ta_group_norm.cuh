@@ -308,12 +308,85 @@ __device__ __forceinline__ float2 load_rank(const float2 *ptr, int rank)
     return v;
 }
 
+template <int BYTES> __device__ __forceinline__ void copy_async(void *shared, const void *global)
+{
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(shared)), "l"(global) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(shared)), "l"(global), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
 // The second launch of a pass may start while the first one ends (programmatic dependent launch): what
 // does not depend on the first is fetched before gn_wait_first().
 __device__ __forceinline__ void gn_allow_second() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void gn_wait_first() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-constexpr int kGnUnroll = 4;            // rows a thread has in flight
+// Rows on their way into a thread's own ring in shared memory: N tensors, D rows ahead.  Nothing but the thread's own
+// cp.async groups orders the copies, so every thread has D rows in flight all the time and no registers hold them.
+template <typename T, int V, int N, int D> struct GnStream {
+    using Vec = Pack<T, V>;
+    static constexpr int kBytes = N * D * kGnThreads * (int)sizeof(Vec);
+    Vec *ring;
+    const T *src[N];
+    long long step;
+    int count, next;
+    static constexpr bool kAsync = sizeof(Vec) >= 4;      // cp.async moves four bytes at least; two-byte vectors are loaded four rows at a time
+    __device__ __forceinline__ void fetch()
+    {
+        if (next < count) {
+#pragma unroll
+            for (int t = 0; t < N; ++t) {
+                copy_async<sizeof(Vec)>(ring + ((next & (D - 1)) * N + t) * kGnThreads, src[t]);
+                src[t] += step;
+            }
+        }
+        ++next;
+        copy_commit();
+    }
+    __device__ __forceinline__ void start(void *shared, long long row_step, int rows)
+    {
+        ring = static_cast<Vec *>(shared) + threadIdx.x;
+        step = row_step;
+        count = rows;
+        next = 0;
+        if constexpr (kAsync) {
+#pragma unroll
+            for (int i = 0; i < D; ++i) fetch();
+        } else if (count > 0) ring[0].load(src[0]);       // (the first row, for those who look at it)
+    }
+    // the first row has arrived
+    __device__ __forceinline__ void wait() const { if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory"); }
+    // f(the row's vectors), row by row
+    template <typename F> __device__ __forceinline__ void run(F f)
+    {
+        if constexpr (kAsync) {
+            for (int i = 0; i < count; ++i) {
+                wait();
+                Vec v[N];
+#pragma unroll
+                for (int t = 0; t < N; ++t) v[t] = ring[((i & (D - 1)) * N + t) * kGnThreads];
+                fetch();
+                f(v);
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        } else {
+            for (int i = 0; i < count; i += 4) {
+                Vec v[4][N];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (i + u < count) {
+#pragma unroll
+                        for (int t = 0; t < N; ++t) v[u][t].load(src[t] + (i + u) * step);
+                    }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (i + u < count) f(v[u]);
+            }
+        }
+    }
+};
+constexpr int kGnAhead = 8, kGnAheadGrad = 4;
 
 // ----------------------------------------------------------------------------- forward
 // Sums of differences to the group's pivot (negated in pv) and of their squares, per channel
@@ -342,72 +415,57 @@ template <int P, typename Vec> __device__ __forceinline__ void add_values(const 
     for (int j = 0; j < P; ++j) sm[j] = add2(sm[j], f[j]);
 }
 
-// Per (sample, group, chunk): mean and sum of squared deviations from it.  The block takes the mean of its first
-// rows as pivot and sums differences to it and their squares.  The share of the pivot's rows is at
-// least 1 / 512 of the block's, so its distance to the block's mean is at most 23 spreads, and as a rule far below one:
-// the difference of sums at the end loses next to nothing however far from zero the values lie.
+// Per (sample, group, chunk): mean and sum of squared deviations from it.
+//
+// The pivot of a group: the mean of its first channel in the block's first rows, up to eight.  Sums of differences to it
+// and of their squares lose count / 8 x 2^-24 of the variance at the very worst (a pivot made of the group's only
+// outlier), as a rule a few 2^-24, however far from zero the values lie.
 template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_stats_kernel(const GnArgs a, const GnShape s)
+__global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_stats_kernel(const __grid_constant__ GnArgs a, const __grid_constant__ GnShape s)
 {
     gn_allow_second();
+    extern __shared__ __align__(16) unsigned char smem[];  // the ring; afterwards [row slot][folded channel]
+    constexpr int P = Pack<T, V>::P;
     const GnPlace at(a, s, blockIdx.x);
     const int count = at.count(s);
-    constexpr int P = Pack<T, V>::P;
-    __shared__ float2 red[kGnThreads * V];                // [row slot][folded channel]
-    __shared__ float pivot[kGnThreads * V];               // [group]
+    GnStream<T, V, 1, kGnAhead> rows;
+    rows.src[0] = (const T *)a.x + (at.n * a.rows + at.row0 + at.r) * a.channels + at.vec * V;
+    rows.start(smem, (long long)s.rows_per_step * a.channels, count);
     const int per_vec = V / s.fold, stride = s.tile * per_vec, groups = at.groups(a, s);
     const int width = s.split == 1 ? s.columns.width : at.width(s) * per_vec;
-    float2 *slot = red + at.r * stride + at.v * per_vec;
-    const bool holds = at.r < s.rows_per_step;
-    const int per_pass = kGnThreads / s.columns.lanes, lane = threadIdx.x & (s.columns.lanes - 1), mine = threadIdx.x / (unsigned)s.columns.lanes;
-    const T *ptr = (const T *)a.x + (at.n * a.rows + at.row0 + at.r) * a.channels + at.vec * V;
-    const long long step = (long long)s.rows_per_step * a.channels;
+    const int sample_rows = min(min(8, s.rows_per_step), at.rows);
+    const float sample_inv = 1.0f / (float)sample_rows;
+    const auto pivot_of = [&](int g) {                    // (the first row slots lie side by side: thread t has vector t)
+        const T *first = reinterpret_cast<const T *>(smem) + g * a.cpg;
+        float t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < sample_rows) t += FeatElem<T>::to_f(first[k * s.tile * V]);
+        return t * sample_inv;
+    };
     float2 pv[P], sm[P], s2[P];
-#pragma unroll
-    for (int j = 0; j < P; ++j) pv[j] = sm[j] = s2[j] = both(0.0f);
-    Pack<T, V> p[kGnUnroll];
-#pragma unroll
-    for (int u = 0; u < kGnUnroll; ++u)
-        if (u < count) p[u].load(ptr + u * step);
-#pragma unroll
-    for (int u = 0; u < kGnUnroll; ++u)
-        if (u < count) add_values<P>(p[u], sm);
-    if (holds) store_folded<V>(slot, sm, s2, s.fold);
-    __syncthreads();
-    const float first_inv = 1.0f / ((float)min(at.rows, kGnUnroll * s.rows_per_step) * (float)(width * s.fold));
-    for (int base = 0; base < groups; base += per_pass) {
-        const int g = base + mine;
-        const float2 t = group_sum(s.columns, red, stride, s.rows_per_step, width, g, g < groups);
-        if (g < groups && lane == 0) pivot[g] = t.x * first_inv;
-    }
+    rows.wait();
     __syncthreads();
     const int group = at.active ? (at.vec * V) / a.cpg - at.group0 : 0;
-    spread_groups<V>(group, at.active ? a.cpg - (at.vec * V) % a.cpg : V, a.cpg, [&](int g) { return make_float2(-pivot[g], 0.0f); }, pv, sm);
+    spread_groups<V>(group, at.active ? a.cpg - (at.vec * V) % a.cpg : V, a.cpg, [&](int g) { return make_float2(-pivot_of(g), 0.0f); }, pv, sm);
+    const int lanes = s.columns.lanes, per_pass = kGnThreads / lanes, lane = threadIdx.x & (lanes - 1), mine = threadIdx.x / (unsigned)lanes;
+    constexpr int kSums = kGnThreads * V * (int)sizeof(float2), kRing = GnStream<T, V, 1, kGnAhead>::kBytes;
+    float *pivots = reinterpret_cast<float *>(smem + (kRing > kSums ? kRing : kSums));          // [groups]
+    for (int g = threadIdx.x; g < groups; g += kGnThreads) pivots[g] = pivot_of(g);
 #pragma unroll
-    for (int u = 0; u < kGnUnroll; ++u)
-        if (u < count) add_moments<P>(p[u], pv, sm, s2);
-    int i = kGnUnroll;
-    ptr += kGnUnroll * step;
-    for (; i + kGnUnroll <= count; i += kGnUnroll, ptr += kGnUnroll * step) {
-#pragma unroll
-        for (int u = 0; u < kGnUnroll; ++u) p[u].load(ptr + u * step);
-#pragma unroll
-        for (int u = 0; u < kGnUnroll; ++u) add_moments<P>(p[u], pv, sm, s2);
-    }
-#pragma unroll
-    for (int u = 0; u < kGnUnroll - 1; ++u)
-        if (i + u < count) p[u].load(ptr + u * step);
-#pragma unroll
-    for (int u = 0; u < kGnUnroll - 1; ++u)
-        if (i + u < count) add_moments<P>(p[u], pv, sm, s2);
-    if (holds) store_folded<V>(slot, sm, s2, s.fold);
+    for (int j = 0; j < P; ++j) s2[j] = both(0.0f);
+    __syncthreads();                                      // the first row may be overwritten now
+    rows.run([&](Pack<T, V> (&x)[1]) { add_moments<P>(x[0], pv, sm, s2); });
+    __syncthreads();
+    float2 *red = reinterpret_cast<float2 *>(smem);
+    if (at.r < s.rows_per_step) store_folded<V>(red + at.r * stride + at.v * per_vec, sm, s2, s.fold);
     __syncthreads();
     const float inv = 1.0f / ((float)at.rows * (float)(width * s.fold));
     for (int base = 0; base < groups; base += per_pass) {
         const int g = base + mine;
         const float2 t = group_sum(s.columns, red, stride, s.rows_per_step, width, g, g < groups);
         if (g < groups && lane == 0)
-            a.part[(((long long)at.n * a.groups + at.group0 + g) * s.chunks + at.chunk) * s.split + at.piece] = moments_of(pivot[g], t, inv);
+            a.part[(((long long)at.n * a.groups + at.group0 + g) * s.chunks + at.chunk) * s.split + at.piece] = moments_of(pivots[g], t, inv);
     }
 }
 
@@ -426,46 +484,42 @@ __device__ __forceinline__ void gn_finish_stats(const GnArgs &a, const GnShape &
         const bool valid = g < groups;
         const long long id = (long long)at.n * a.groups + at.group0 + g;
         const float2 *part = a.part + id * entries;
-        // the lane's first eight entries stay in registers for the second sum
-        float2 p[8];
-        float n[8], m = 0.0f, q = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int e = lane + i * lanes;
-            const bool have = valid && e < entries;
-            p[i] = have ? __ldcg(part + e) : make_float2(0.0f, 0.0f);
-            n[i] = have ? values(e) : 0.0f;
-            m = fmaf(n[i], p[i].x, m);
-        }
-        if (valid)
-            for (int e = lane + 8 * lanes; e < entries; e += lanes) m = fmaf(values(e), __ldcg(part + e).x, m);
-        m = __shfl_sync(0xffffffffu, lane_sum(m, lanes) * inv, 0, lanes);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (n[i] > 0.0f) q += fmaf(n[i] * (p[i].x - m), p[i].x - m, p[i].y);
-        if (valid)
-            for (int e = lane + 8 * lanes; e < entries; e += lanes) {
-                const float2 t = __ldcg(part + e);
-                q += fmaf(values(e) * (t.x - m), t.x - m, t.y);
+        // Sums of the distances to the first chunk's mean and of their squares: it holds at least 1 / 1024 of the values, so its
+        // mean is at most 32 spreads off, and as a rule a fraction of one.
+        float2 t = make_float2(0.0f, 0.0f);
+        float ref = 0.0f;
+        if (valid) {
+            ref = __ldcg(part).x;
+#pragma unroll 4
+            for (int e = lane; e < entries; e += lanes) {
+                const float2 p = __ldcg(part + e);
+                const float n = values(e), d = p.x - ref;
+                t = add2(t, make_float2(n * d, fmaf(n * d, d, p.y)));
             }
-        q = lane_sum(q, lanes);
+        }
+        t = lane_sum(t, lanes);
+        const float2 mq = moments_of(ref, t, inv);
         if (valid && lane == 0) {
-            const float rstd = rsqrtf(q * inv + a.eps);
-            stat[g] = make_float2(m, rstd);
-            if (at.chunk == 0 && at.piece == 0) { a.mean[id] = m; a.rstd[id] = rstd; }
+            const float rstd = rsqrtf(mq.y * inv + a.eps);
+            stat[g] = make_float2(mq.x, rstd);
+            if (at.chunk == 0 && at.piece == 0) { a.mean[id] = mq.x; a.rstd[id] = rstd; }
         }
     }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_apply_kernel(const GnArgs a, const GnShape s)
+__global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_apply_kernel(const __grid_constant__ GnArgs a, const __grid_constant__ GnShape s)
 {
-    extern __shared__ float2 stat[];                      // [groups_per_tile] (mean, rstd)
+    extern __shared__ __align__(16) unsigned char smem[];  // the ring, then
+    using Rows = GnStream<T, V, 1, kGnAhead>;
+    float2 *stat = reinterpret_cast<float2 *>(smem + Rows::kBytes);       // [groups_per_tile] (mean, rstd)
     const GnPlace at(a, s, gridDim.x - 1 - blockIdx.x);        // what was read last comes first: it is in L2
     const int count = at.count(s), c0 = at.vec * V;
     const long long first = (at.n * a.rows + at.row0 + at.r) * a.channels + c0, step = (long long)s.rows_per_step * a.channels;
-    const T *src = (const T *)a.x + first;
     T *dst = (T *)a.y + first;
+    Rows rows;                                            // (x is not written by the first launch)
+    rows.src[0] = (const T *)a.x + first;
+    rows.start(smem, step, count);
     constexpr int P = Pack<T, V>::P;
     float2 mean[P], scale[P], bias[P], rstd[P];
     load_params<V>(a.weight, a.param_code, a.wide_params, c0, at.active, 1.0f, scale);
@@ -478,27 +532,16 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_apply_kernel(
 #pragma unroll
     for (int j = 0; j < P; ++j) scale[j] = mul2(scale[j], rstd[j]);
     with_activation(a.act, [&](auto act) {
-        const auto apply = [&](Pack<T, V> &p, T *out) {
+        rows.run([&](Pack<T, V> (&x)[1]) {
             float2 f[P];
-            p.unpack(f);
+            x[0].unpack(f);
 #pragma unroll
             for (int j = 0; j < P; ++j) f[j] = fma2(add2(f[j], mean[j]), scale[j], bias[j]);
             activate<decltype(act)::value, sizeof(T) == 2, P>(f);
-            p.pack(f);
-            p.store(out);
-        };
-        Pack<T, V> p[kGnUnroll];
-        int i = 0;
-        for (; i + kGnUnroll <= count; i += kGnUnroll, src += kGnUnroll * step, dst += kGnUnroll * step) {
-#pragma unroll
-            for (int u = 0; u < kGnUnroll; ++u) p[u].load_stream(src + u * step);
-#pragma unroll
-            for (int u = 0; u < kGnUnroll; ++u) apply(p[u], dst + u * step);
-        }
-        for (; i < count; ++i, src += step, dst += step) {
-            p[0].load_stream(src);
-            apply(p[0], dst);
-        }
+            x[0].pack(f);
+            x[0].store(dst);
+            dst += step;
+        });
     });
 }
 
@@ -531,13 +574,14 @@ __device__ __forceinline__ void sum_columns(float2 *acc, int stride, int columns
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_sums_kernel(const GnArgs a, const GnShape s)
+__global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_sums_kernel(const __grid_constant__ GnArgs a, const __grid_constant__ GnShape s)
 {
     gn_allow_second();
     const GnPlace at(a, s, blockIdx.x);
     const int count = at.count(s), c0 = at.vec * V;
-    constexpr int P = Pack<T, V>::P, U = kGnUnroll / 2;
-    __shared__ float2 acc[kGnThreads * V];                // [row slot][folded channel], then [row slot][channel]
+    constexpr int P = Pack<T, V>::P;
+    extern __shared__ __align__(16) unsigned char smem[];  // the ring; afterwards
+    float2 *acc = reinterpret_cast<float2 *>(smem);       // [row slot][folded channel], then [row slot][channel]
     {
         const long long g0 = (long long)at.n * a.groups;
         float2 mean[P], scale[P], bias[P], rstd[P], sgx[P], sg[P];
@@ -548,32 +592,23 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_sums_ke
 #pragma unroll
         for (int j = 0; j < P; ++j) { scale[j] = mul2(scale[j], rstd[j]); sgx[j] = sg[j] = both(0.0f); }
         const long long first = (at.n * a.rows + at.row0 + at.r) * a.channels + c0, step = (long long)s.rows_per_step * a.channels;
-        const T *px = (const T *)a.x + first, *pd = (const T *)a.dy + first;
+        GnStream<T, V, 2, kGnAheadGrad> rows;
+        rows.src[0] = (const T *)a.x + first;
+        rows.src[1] = (const T *)a.dy + first;
+        rows.start(smem, step, count);
         with_activation(a.act, [&](auto act) {
-            const auto add = [&](const Pack<T, V> &x, const Pack<T, V> &d) {
+            rows.run([&](Pack<T, V> (&x)[2]) {
                 float2 f[P], z[P], g[P];
-                x.unpack(f);
-                d.unpack(g);
+                x[0].unpack(f);
+                x[1].unpack(g);
 #pragma unroll
                 for (int j = 0; j < P; ++j) { f[j] = add2(f[j], mean[j]); z[j] = fma2(f[j], scale[j], bias[j]); }
                 activate_grad<decltype(act)::value, sizeof(T) == 2, P>(z, g);
 #pragma unroll
                 for (int j = 0; j < P; ++j) { sg[j] = add2(sg[j], g[j]); sgx[j] = fma2(g[j], f[j], sgx[j]); }
-            };
-            Pack<T, V> x[U], d[U];
-            int i = 0;
-            for (; i + U <= count; i += U, px += U * step, pd += U * step) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) { x[u].load(px + u * step); d[u].load(pd + u * step); }
-#pragma unroll
-                for (int u = 0; u < U; ++u) add(x[u], d[u]);
-            }
-            for (; i < count; ++i, px += step, pd += step) {
-                x[0].load(px);
-                d[0].load(pd);
-                add(x[0], d[0]);
-            }
+            });
         });
+        __syncthreads();
         // sums of (u xhat, rstd u) of the groups: u xhat = g scale (x - mean)
         const int per_vec = V / s.fold, stride = s.tile * per_vec, groups = at.groups(a, s), lanes = s.columns.lanes, lane = threadIdx.x & (lanes - 1);
         const int width = s.split == 1 ? s.columns.width : at.width(s) * per_vec;
@@ -640,12 +675,19 @@ static __global__ void __launch_bounds__(kGnThreads) gn_grad_params_kernel(const
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_input_kernel(const GnArgs a, const GnShape s)
+__global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_input_kernel(const __grid_constant__ GnArgs a, const __grid_constant__ GnShape s)
 {
-    extern __shared__ float2 stat[];                      // [groups_per_tile] means of (u xhat, rstd u)
+    extern __shared__ __align__(16) unsigned char smem[];  // the ring, then
+    using Rows = GnStream<T, V, 2, kGnAheadGrad>;
+    float2 *stat = reinterpret_cast<float2 *>(smem + Rows::kBytes);       // [groups_per_tile] means of (u xhat, rstd u)
     const GnPlace at(a, s, gridDim.x - 1 - blockIdx.x);
     const int count = at.count(s), c0 = at.vec * V;
-    constexpr int P = Pack<T, V>::P, U = kGnUnroll / 2;
+    constexpr int P = Pack<T, V>::P;
+    const long long first = (at.n * a.rows + at.row0 + at.r) * a.channels + c0, step = (long long)s.rows_per_step * a.channels;
+    Rows rows;                                            // (x and dy are not written by the first launch)
+    rows.src[0] = (const T *)a.x + first;
+    rows.src[1] = (const T *)a.dy + first;
+    rows.start(smem, step, count);
     const long long g0 = (long long)at.n * a.groups;
     float2 mean[P], scale[P], bias[P], rstd[P], m_ux[P], m_u[P];
     load_params<V>(a.weight, a.param_code, a.wide_params, c0, at.active, 1.0f, scale);
@@ -673,35 +715,21 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_input_k
     spread_groups<V>(group - at.group0, left, a.cpg, [&](int g) { return make_float2(-stat[g].x, -stat[g].y); }, m_ux, m_u);
 #pragma unroll
     for (int j = 0; j < P; ++j) m_ux[j] = mul2(m_ux[j], mul2(rstd[j], rstd[j]));       // dx = g scale - ((x - mean) m_ux + m_u)
-    const long long first = (at.n * a.rows + at.row0 + at.r) * a.channels + c0, step = (long long)s.rows_per_step * a.channels;
-    const T *px = (const T *)a.x + first, *pd = (const T *)a.dy + first;
     T *out = (T *)a.dx + first;
     with_activation(a.act, [&](auto act) {
-        const auto apply = [&](const Pack<T, V> &x, Pack<T, V> &d, T *to) {
+        rows.run([&](Pack<T, V> (&x)[2]) {
             float2 f[P], z[P], g[P];
-            x.unpack(f);
-            d.unpack(g);
+            x[0].unpack(f);
+            x[1].unpack(g);
 #pragma unroll
             for (int j = 0; j < P; ++j) { f[j] = add2(f[j], mean[j]); z[j] = fma2(f[j], scale[j], bias[j]); }
             activate_grad<decltype(act)::value, sizeof(T) == 2, P>(z, g);
 #pragma unroll
             for (int j = 0; j < P; ++j) g[j] = fma2(g[j], scale[j], fma2(f[j], m_ux[j], m_u[j]));
-            d.pack(g);
-            d.store(to);
-        };
-        Pack<T, V> x[U], d[U];
-        int i = 0;
-        for (; i + U <= count; i += U, px += U * step, pd += U * step, out += U * step) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) { x[u].load_stream(px + u * step); d[u].load_stream(pd + u * step); }
-#pragma unroll
-            for (int u = 0; u < U; ++u) apply(x[u], d[u], out + u * step);
-        }
-        for (; i < count; ++i, px += step, pd += step, out += step) {
-            x[0].load_stream(px);
-            d[0].load_stream(pd);
-            apply(x[0], d[0], out);
-        }
+            x[1].pack(g);
+            x[1].store(out);
+            out += step;
+        });
     });
 }
 
@@ -742,18 +770,18 @@ template <typename T, int V> cudaError_t gn_launch_streaming(const GnArgs &all, 
 {
     GnArgs a = all;
     const GnShape s = gn_shape(a, V, backward);
-    const size_t smem = s.groups_per_tile * sizeof(float2);
+    const size_t stat = s.groups_per_tile * sizeof(float2), sums = kGnThreads * V * sizeof(float2);
+    constexpr size_t ring = GnStream<T, V, 1, kGnAhead>::kBytes, grad_ring = GnStream<T, V, 2, kGnAheadGrad>::kBytes;
     const dim3 grid((unsigned)(a.n * s.chunks), s.tiles);
     cudaError_t e;
     if (!backward) {
-        e = gn_launch_kernel(gn_stats_kernel<T, V>, grid, 0, false, stream, a, s);
-        return e != cudaSuccess ? e : gn_launch_kernel(gn_apply_kernel<T, V>, grid, smem, true, stream, a, s);
+        e = gn_launch_kernel(gn_stats_kernel<T, V>, grid, (ring > sums ? ring : sums) + stat, false, stream, a, s);
+        return e != cudaSuccess ? e : gn_launch_kernel(gn_apply_kernel<T, V>, grid, ring + stat, true, stream, a, s);
     }
     a.channel_part = gn_channel_part(a, s);
-    e = gn_launch_kernel(gn_grad_sums_kernel<T, V>, grid, 0, false, stream, a, s);
-    if (e == cudaSuccess && a.dx) e = gn_launch_kernel(gn_grad_input_kernel<T, V>, grid, smem, true, stream, a, s);
-    if (e == cudaSuccess && (a.dweight || a.dbias))
-        e = gn_launch_params(a, a.channel_part, a.n * s.chunks, stream);
+    e = gn_launch_kernel(gn_grad_sums_kernel<T, V>, grid, grad_ring > sums ? grad_ring : sums, false, stream, a, s);
+    if (e == cudaSuccess && a.dx) e = gn_launch_kernel(gn_grad_input_kernel<T, V>, grid, grad_ring + stat, true, stream, a, s);
+    if (e == cudaSuccess && (a.dweight || a.dbias)) e = gn_launch_params(a, a.channel_part, a.n * s.chunks, stream);
     return e;
 }
 

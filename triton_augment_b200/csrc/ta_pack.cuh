@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "ta_features.h"
 
 namespace ta {
@@ -41,8 +43,9 @@ template <> struct RawOf<16> { using type = uint4; };
 // V elements, V * sizeof(T) in {2, 4, 8, 16} bytes and aligned to that
 template <typename T, int V> struct Pack {
     using Raw = typename RawOf<V * sizeof(T)>::type;
-    union { Raw raw; T v[V]; typename FeatElem<T>::Pair p[V > 1 ? V / 2 : 1]; };
-    __device__ __forceinline__ Pack() {}
+    using Half = std::conditional_t<(V > 1), typename FeatElem<T>::Pair, T>;       // (a pair would make a single element as large as two)
+    union { Raw raw; T v[V]; Half p[V > 1 ? V / 2 : 1]; };
+    __device__ __forceinline__ Pack() { static_assert(sizeof(Pack) == V * sizeof(T), "a vector is its elements"); }
     __device__ __forceinline__ Pack(const Pack &o) : raw(o.raw) {}
     __device__ __forceinline__ Pack &operator=(const Pack &o) { raw = o.raw; return *this; }
     __device__ __forceinline__ void load(const T *ptr) { raw = *reinterpret_cast<const Raw *>(ptr); }
