@@ -142,7 +142,8 @@ def _gn(**kw):
 @pytest.mark.parametrize("kw, code", [
     (dict(struct_size=8), -2), (dict(dtype=_lib.U8), -3), (dict(weight=4096, param_dtype=7), -3), (dict(activation=9), -4),
     (dict(groups=3), -2), (dict(groups=0), -2), (dict(n=-1), -2), (dict(eps=-1.0), -2), (dict(n=1 << 22), -8),
-    (dict(rows=1 << 31), -8), (dict(x=None), -1), (dict(mean=None), -1), (dict(x=4097), -4),
+    (dict(rows=1 << 31), -8), (dict(x=None), -1), (dict(mean=None), -1), (dict(x=4097), -4), (dict(mean=4098), -4), (dict(weight=4098), -4),
+    (dict(channels=1 << 21, groups=1), -8),
 ])
 def test_group_norm_abi_refusals(kw, code):
     assert _lib.load().ta_b200_group_norm(C.byref(_gn(**kw)), None) == code
@@ -166,7 +167,7 @@ def _dr(**kw):
 
 @pytest.mark.parametrize("kw, code", [
     (dict(struct_size=8), -2), (dict(dtype=_lib.U8_F16), -3), (dict(p=1.01), -4), (dict(p=float("nan")), -4),
-    (dict(sizes=(1, 1, -1, 8)), -2), (dict(sizes=(1 << 20, 1 << 20, 1 << 20, 1)), -8), (dict(x=None), -1), (dict(y=None), -1),
+    (dict(sizes=(1, 1, -1, 8)), -2), (dict(sizes=(1 << 14, 1 << 14, 1 << 14, 1)), -8), (dict(x=None), -1), (dict(y=None), -1),
     (dict(x=4097), -4), (dict(seed_ptr=4100), -4),
 ])
 def test_dropout_abi_refusals(kw, code):
@@ -196,7 +197,7 @@ def _ro(**kw):
     (dict(dim=600, sections=(300, 300, 0)), -8), (dict(dim=1 << 17), -8), (dict(base=0.0), -4), (dict(pairing=2), -4),
     (dict(spectrum=2), -4), (dict(position_kind=4), -4), (dict(grid=(2, 2, 0)), -2), (dict(grid=(-2, -3, 0)), -2), (dict(patch=0.0), -4),
     (dict(axes=1, sections=(8, 0, 0), grid=(6, 0, 0), top=4096), -4), (dict(q=None), -1), (dict(k_heads=1), -1),
-    (dict(position_kind=1), -1), (dict(position_kind=1, positions=4100), -4), (dict(q=4097), -4),
+    (dict(position_kind=1), -1), (dict(position_kind=1, positions=4100), -4), (dict(q=4097), -4), (dict(top=4097), -4), (dict(tokens=1 << 31, position_kind=1), -8),
 ])
 def test_rotary_abi_refusals(kw, code):
     assert _lib.load().ta_b200_rotary(C.byref(_ro(**kw)), None) == code
@@ -248,3 +249,19 @@ def test_reference_group_norm_against_torch_and_differences():
         r = R.group_norm(x, 3, w, b, 1e-5, act, dy=dy)
         for name, want in zip(("y", "dx", "dweight", "dbias"), (y.detach(), *grads)):
             assert float((r[name] - want).abs().max()) < 1e-12, (act, name)
+
+
+def test_rotary_configuration_is_kept_by_value():
+    """A number held in a tensor is read at every call; a size that is no integer is refused, not cut."""
+    from triton_augment_b200 import _functional_features as FF
+    q = torch.zeros(1, 4, 1, 8)
+    patch, before = torch.tensor(2.0), len(FF._ROTARY_CACHE)
+    for value in (3.25, 5.75):
+        patch.fill_(value)
+        with pytest.raises(ValueError, match="CUDA"):
+            ta.rotary_embedding(q, sections=(4, 4), grid=(2, 2), patch=patch)
+    assert len(FF._ROTARY_CACHE) == min(64, before + 2)
+    assert all(type(v) in (float, int, str, tuple, type(None)) for key in FF._ROTARY_CACHE for v in key)
+    for kw in (dict(sections=(4.5, 4)), dict(sections=(4, 4), prefix=0.5), dict(sections=(4, 4), grid=(2.0, 2))):
+        with pytest.raises(TypeError):
+            ta.rotary_embedding(q, **{"grid": (2, 2), **kw})

@@ -99,9 +99,9 @@ def test_gradients(mode, dtype):
     # linear in x and in the residual: a difference of two calls is the gradient's product
     if dtype == torch.float32:
         d = _randn(shape, dtype, 4)
-        num = (ta.dropout(x + d, 0.2, 42, mode=mode).double() - ta.dropout(x, 0.2, 42, mode=mode).double()).mul(dy.double()).sum()
+        num = (ta.dropout((x + d).detach(), 0.2, 42, mode=mode).double() - ta.dropout(x.detach(), 0.2, 42, mode=mode).double()).mul(dy.double()).sum()
         ana = (dx.double() * d.double()).sum()
-        assert abs(float(num - ana)) <= 8 * R.U * float((dy.abs() * (x.abs() + d.abs())).double().sum()) / 0.8
+        assert abs(float(num - ana)) <= 8 * R.U * float((dy.abs() * (x.detach().abs() + d.abs())).double().sum()) / 0.8
     expanded = torch.autograd.grad(ta.dropout(x, 0.2, 42, mode=mode).sum(), x)[0]
     want, tol = _expect(torch.ones_like(x), keep, 0.2)
     R.assert_within(expanded, want, tol, "expanded dy")
@@ -142,6 +142,36 @@ def test_entries_beyond_32_bits():
         keep = torch.from_numpy(R.mask_numbers(24, 3, first=first) >= 2 ** 31).to(DEV)
         assert torch.equal(got[first:first + 24] != 0, keep)
     del x, got
+    torch.cuda.empty_cache()
+
+
+def test_shared_masks_beyond_32_bits():
+    """Two samples of 2^31 + 8 halves under one mask, and a mask entry per sample: the general index arithmetic in 64 bits."""
+    plane = 2 ** 31 + 8
+    x = torch.ones(2, 1, 1, plane, dtype=torch.float16, device=DEV)
+    got = ta.dropout(x, 0.5, 3, same_on_batch=True)
+    for first in (0, plane - 24):
+        keep = torch.from_numpy(R.mask_numbers(24, 3, first=first) >= 2 ** 31).to(DEV)
+        for n in (0, 1):
+            assert torch.equal(got[n, 0, 0, first:first + 24] != 0, keep)
+    del got
+    got = ta.dropout(x, 0.5, 3, mode="sample")
+    keep = R.mask_numbers(2, 3) >= 2 ** 31
+    for n in (0, 1):
+        assert bool((got[n, 0, 0, ::65537] != 0).all()) == bool(keep[n]) and bool((got[n, 0, 0, -9:] != 0).any()) == bool(keep[n])
+    del x, got
+    torch.cuda.empty_cache()
+
+
+def test_rows_next_to_the_32_bit_limit():
+    """The row kernel hands over to the general one before an index of its last block could wrap."""
+    for numel in (2 ** 32 - 2 ** 15, 2 ** 32 - 8):
+        x = torch.ones(1, 1, 2, numel // 2, dtype=torch.float16, device=DEV).permute(0, 2, 1, 3).contiguous()        # two channels
+        got = ta.dropout(x, 0.5, 7, mode="channel")
+        keep = R.mask_numbers(2, 7) >= 2 ** 31
+        for c in (0, 1):
+            assert bool((got[0, c, 0, ::65537] != 0).all()) == bool(keep[c]) and bool((got[0, c, 0, -4097:] != 0).any()) == bool(keep[c])
+        del x, got
     torch.cuda.empty_cache()
 
 

@@ -82,3 +82,46 @@ def test_block_in_16_bits_runs_and_repeats(dtype):
         results.append([loss.detach()] + list(torch.autograd.grad(loss, leaves)))
     assert all(bool(torch.isfinite(t).all()) and bool(t.any()) for t in results[0])
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][2], results[1][2])
+
+
+def _calls():
+    w = torch.ones(16, device="cuda")
+    grid = dict(sections=(4, 4), grid=(2, 2))
+    return {"group_norm": ((2, 16, 6, 6), lambda x: ta.group_norm(x, 4, w, activation="silu")),
+            "dropout": ((2, 16, 6, 6), lambda x: ta.dropout(x, 0.3, 5)),
+            "rotary": ((2, 4, 3, 8), lambda x: ta.rotary_embedding(x, **grid))}
+
+
+@pytest.mark.parametrize("name", ["group_norm", "dropout", "rotary"])
+def test_negated_views(name):
+    """Tensors whose values torch keeps negated, features and gradients alike."""
+    shape, f = _calls()[name]
+    x, dy = torch.randn(shape, device="cuda"), torch.randn(shape, device="cuda")
+    plain = (-x).requires_grad_()
+    neg = torch._neg_view(x).requires_grad_()
+    assert neg.is_neg()
+    a, b = f(plain), f(neg)
+    assert torch.equal(a, b)
+    assert torch.equal(torch.autograd.grad(a, plain, -dy)[0], torch.autograd.grad(b, neg, torch._neg_view(dy))[0])
+
+
+@pytest.mark.parametrize("name", ["group_norm", "dropout", "rotary"])
+def test_forward_mode_is_refused(name):
+    import torch.autograd.forward_ad as fw
+    shape, f = _calls()[name]
+    with fw.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        f(fw.make_dual(torch.randn(shape, device="cuda"), torch.randn(shape, device="cuda")))
+
+
+@pytest.mark.parametrize("name", ["group_norm", "dropout", "rotary"])
+def test_threads_share_a_graph(name):
+    """Four threads go backward through one graph, and through graphs of their own."""
+    from concurrent.futures import ThreadPoolExecutor
+    shape, f = _calls()[name]
+    x, dy = torch.randn(shape, device="cuda").requires_grad_(), torch.randn(shape, device="cuda")
+    y = f(x)
+    want = torch.autograd.grad(y, x, dy, retain_graph=True)[0]
+    with ThreadPoolExecutor(4) as pool:
+        got = list(pool.map(lambda i: torch.autograd.grad(y if i % 2 else f(x), x, dy, retain_graph=True)[0], range(32)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)

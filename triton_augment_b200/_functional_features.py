@@ -2,7 +2,7 @@
 
 ``group_norm`` (channels-last features, with an activation), ``dropout`` (mask computed from a counter,
 never stored) and ``rotary_embedding`` (positions with one to three axes).  float32, float16 and
-bfloat16 CUDA tensors, differentiable once; each call is one call into libta_b200.so on torch's
+bfloat16 CUDA tensors, differentiable once (backward mode only); each call is one call into libta_b200.so on torch's
 current stream.  No counterpart in the reference.
 
 A CUDA graph may hold forward and backward of these operators.  As with any torch operator, no graph
@@ -13,6 +13,7 @@ of the eager call.
 from __future__ import annotations
 
 import math
+from operator import index
 
 import torch
 
@@ -163,21 +164,18 @@ class _Rotary:
     __slots__ = ("sections", "grid", "prefix", "call")
 
     def __init__(self, sections, grid, patch, base, pairing, spectrum, prefix):
-        self.sections = tuple(int(s) for s in sections)
+        self.sections = sections
         axes = len(self.sections)
         if not 1 <= axes <= 3:
             raise ValueError(f"sections must name one to three axes, got {axes}")
         if any(s < 0 or s % 2 for s in self.sections) or sum(self.sections) > 512:
             raise ValueError(f"sections must be even, not negative, and add up to at most 512, got {self.sections}")
-        base = float(base)
         if not 0.0 < base < float("inf"):
             raise ValueError(f"base must be positive, got {base}")
         pairing, spectrum = _choice(pairing, _lib.PAIRINGS, "pairing"), _choice(spectrum, _lib.SPECTRA, "spectrum")
-        self.prefix = int(prefix)
-        self.grid = None
-        patch = float(patch)
+        self.prefix = prefix
+        self.grid = grid
         if grid is not None:
-            self.grid = tuple(int(g) for g in grid)
             if len(self.grid) != axes or any(g < 0 for g in self.grid):
                 raise ValueError(f"grid must have {axes} sizes like sections, got {grid}")
             if not 0.0 < patch < float("inf"):
@@ -243,7 +241,9 @@ def rotary_embedding(q, k=None, *, sections, positions=None, grid=None, patch: f
             raise TypeError(f"k must be {q.dtype} like q, got {k.dtype}")
     if isinstance(grid, int):
         grid = (grid,)
-    spec = _rotary_spec(tuple(sections), None if grid is None else tuple(grid), patch, base, pairing, spectrum, prefix)
+    patch = float(patch)                                  # (numbers only: a tensor in the key would stand for its identity)
+    spec = _rotary_spec(tuple(map(index, sections)), None if grid is None else tuple(map(index, grid)), patch, float(base),
+                        pairing, spectrum, index(prefix))
     axes, prefix = len(spec.sections), spec.prefix
     if sum(spec.sections) > dim:
         raise ValueError(f"sections must be even, not negative, and add up to at most {dim}, got {spec.sections}")

@@ -22,8 +22,8 @@ static int group_norm_args(const ta_b200_group_norm_params *p, bool backward, Gn
         return fail(TA_B200_ERR_SHAPE, "bad sizes n=%lld rows=%lld channels=%d groups=%d (channels must be a multiple of groups)",
                     (long long)p->n, (long long)p->rows, p->channels, p->groups);
     if (!(p->eps >= 0.0f)) return fail(TA_B200_ERR_SHAPE, "eps must not be negative");
-    if (p->n >= (1 << 22) || p->rows >= (1LL << 31) || p->channels > (1 << 20) || (double)p->n * p->rows * p->channels >= 1.0e15)
-        return fail(TA_B200_ERR_TOO_LARGE, "at most 2^22 samples, 2^31 rows and 2^20 channels per call");
+    if (p->n >= (1 << 22) || p->rows >= (1LL << 31) || p->channels > (1 << 20) || (double)p->n * p->rows * p->channels >= 4398046511104.0)
+        return fail(TA_B200_ERR_TOO_LARGE, "at most 2^22 samples, 2^31 rows, 2^20 channels and 2^42 elements per call");
     const bool empty = p->n == 0 || p->rows == 0;
     if (!empty && (!p->x || (backward ? !p->dy || !p->mean || !p->rstd : !p->y || !p->mean || !p->rstd)))
         return fail(TA_B200_ERR_NULL, "x, mean, rstd and y (forward) or dy (backward) are required");
@@ -51,7 +51,8 @@ static int group_norm(const ta_b200_group_norm_params *p, bool backward, cudaStr
     int rc = group_norm_args(p, backward, a);
     if (rc != TA_B200_OK) return rc;
     const size_t es = feature_bytes(p->dtype), pb = feature_bytes(p->param_dtype);
-    if (((uintptr_t)p->x | (uintptr_t)p->y | (uintptr_t)p->dy | (uintptr_t)p->dx) % es)
+    if (((uintptr_t)p->x | (uintptr_t)p->y | (uintptr_t)p->dy | (uintptr_t)p->dx) % es || ((uintptr_t)p->mean | (uintptr_t)p->rstd) % 4 ||
+        (pb && ((uintptr_t)p->weight | (uintptr_t)p->bias | (uintptr_t)p->dweight | (uintptr_t)p->dbias) % pb))
         return fail(TA_B200_ERR_UNSUPPORTED, "tensors must be aligned to their elements");
     if (a.n == 0 || a.rows == 0) {
         // no element: the parameters' gradients are zero
@@ -90,7 +91,7 @@ static int dropout(const ta_b200_dropout_params *p, cudaStream_t stream)
         if (p->sizes[d] < 0) return fail(TA_B200_ERR_SHAPE, "size %d is negative", d);
         total *= (double)p->sizes[d];
     }
-    if (total >= 1.0e15) return fail(TA_B200_ERR_TOO_LARGE, "too many elements");
+    if (total >= 4398046511104.0) return fail(TA_B200_ERR_TOO_LARGE, "at most 2^42 elements per call");
     if (total == 0.0) return TA_B200_OK;
     if (!p->x || !p->y) return fail(TA_B200_ERR_NULL, "x/y is NULL");
     if (((uintptr_t)p->x | (uintptr_t)p->y | (uintptr_t)p->residual) % es || (uintptr_t)p->seed_ptr % 8)
@@ -156,8 +157,8 @@ static int rotary(const ta_b200_rotary_params *p, cudaStream_t stream)
     }
     if (rot > p->dim) return fail(TA_B200_ERR_SHAPE, "sections add up to more than the head dimension %d", p->dim);
     if (rot / 2 > kRotaryMaxPairs) return fail(TA_B200_ERR_TOO_LARGE, "at most %d rotated elements per head", 2 * kRotaryMaxPairs);
-    if (p->tokens >= (1LL << 31) || p->dim > 65536 || p->q_heads > 65536 || p->k_heads > 65536 || (double)p->n * p->tokens * p->dim >= 1.0e15)
-        return fail(TA_B200_ERR_TOO_LARGE, "tokens below 2^31, head dimension and heads up to 65536");
+    if (p->tokens >= (1LL << 31) || p->dim > 65536 || p->q_heads > 65536 || p->k_heads > 65536 || (double)p->n * p->tokens * p->dim >= 4398046511104.0)
+        return fail(TA_B200_ERR_TOO_LARGE, "tokens below 2^31, head dimension and heads up to 65536, 2^42 elements per head");
     if (!(p->base > 0.0)) return fail(TA_B200_ERR_UNSUPPORTED, "base must be positive");
     if (p->pairing != TA_B200_PAIR_INTERLEAVED && p->pairing != TA_B200_PAIR_HALVES) return fail(TA_B200_ERR_UNSUPPORTED, "pairing %d", p->pairing);
     if (p->spectrum != TA_B200_SPECTRUM_AXIS && p->spectrum != TA_B200_SPECTRUM_JOINT)
@@ -180,7 +181,7 @@ static int rotary(const ta_b200_rotary_params *p, cudaStream_t stream)
         return fail(TA_B200_ERR_NULL, "q/k or their outputs are NULL");
     if (p->position_kind != TA_B200_POS_GRID && !p->positions && p->tokens > p->prefix) return fail(TA_B200_ERR_NULL, "positions is NULL");
     if (((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->q_out | (uintptr_t)p->k_out) % es ||
-        (uintptr_t)p->positions % (p->position_kind == TA_B200_POS_I64 ? 8 : 4))
+        (uintptr_t)p->positions % (p->position_kind == TA_B200_POS_I64 ? 8 : 4) || ((uintptr_t)p->top | (uintptr_t)p->left) % 4)
         return fail(TA_B200_ERR_UNSUPPORTED, "tensors must be aligned to their elements");
     DeviceState *s = nullptr;
     int rc = current_device(&s, nullptr);

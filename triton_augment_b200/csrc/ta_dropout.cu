@@ -251,7 +251,7 @@ template <typename T, int KIND> static cudaError_t dropout_launch_kind(const Dro
 }
 
 // One entry for a whole row of neighbours (planes of a channel, channels of a pixel, samples): a block makes the
-// decisions of the rows that it touches once, in shared memory.  16-byte boundaries, fewer than 2^32 elements.
+// decisions of the rows that it touches once, in shared memory.  16-byte boundaries, indices of 32 bits.
 // 64 x 256 x 56^2 float16, channels: a decision per eight elements 65 us, per row with sets of eight per thread 1 / 2 / 3 / 4:
 // 53 / 43 / 42 / 35.5 us (floor 31).
 template <typename T, bool RESIDUAL>
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kDropoutThreads, 4) dropout_rows_kernel(const 
 template <typename T> static cudaError_t dropout_launch(const DropoutArgs &a, cudaStream_t stream)
 {
     const bool wide = (((uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.residual) % 16) == 0;
-    if (wide && a.mstride[3] == 0 && a.numel < (1LL << 32)) {
+    if (wide && a.mstride[3] == 0 && a.numel <= (1LL << 32) - (1 << 15)) {       // (indices up to a block past the end fit 32 bits)
         constexpr int per_block = kDropoutThreads * 8 * (sizeof(T) == 2 ? 4 : 2);
         const unsigned blocks = (unsigned)((a.numel + per_block - 1) / per_block);
         if (a.residual) dropout_rows_kernel<T, true><<<blocks, kDropoutThreads, 0, stream>>>(a);

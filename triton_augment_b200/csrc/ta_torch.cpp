@@ -4,6 +4,8 @@
 // costs tens of microseconds per operator.  The library itself stays free of torch; this file is its client.
 #include <dlfcn.h>
 
+#include <mutex>
+
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -70,9 +72,13 @@ void *address(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 Tensor given(const optional<Tensor> &t) { return t.has_value() ? *t : Tensor(); }
 
+// `t` with its values in memory: a view of a conjugate's imaginary part holds them negated
+Tensor stored(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // `t` with its channels (dimension -3) last in memory and no gaps; `t` itself if it is already
-Tensor channels_last(const Tensor &t)
+Tensor channels_last(const Tensor &given)
 {
+    const Tensor t = stored(given);
     if (t.dim() == 4) return t.contiguous(at::MemoryFormat::ChannelsLast);
     const Tensor last = t.movedim(-3, -1);
     return last.is_contiguous() ? t : last.contiguous().movedim(-1, -3);
@@ -80,6 +86,8 @@ Tensor channels_last(const Tensor &t)
 
 bool wants_grad(std::initializer_list<const Tensor *> ts)
 {
+    for (const Tensor *t : ts)
+        if (t->defined() && t->_fw_grad(0).defined()) throw py::value_error("forward-mode derivatives are not supported");
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor *t : ts)
         if (t->defined() && t->requires_grad()) return true;
@@ -144,6 +152,7 @@ struct GroupNormBackward : Node {
 
     variable_list apply(variable_list &&grads) override
     {
+        const std::lock_guard<std::mutex> lock(mutex_);        // two threads may go backward through one graph
         const Tensor &dy0 = grads[0];
         variable_list out(3);
         if (!dy0.defined()) return out;
@@ -165,6 +174,7 @@ struct GroupNormBackward : Node {
     }
     void release_variables() override
     {
+        const std::lock_guard<std::mutex> lock(mutex_);
         x.reset_data();
         weight.reset_data();
         bias.reset_data();
@@ -183,8 +193,8 @@ Tensor group_norm(const Tensor &x0, const optional<Tensor> &weight0, const optio
     {
         at::AutoGradMode off(false);
         x = channels_last(x0);
-        w = weight.defined() ? weight.contiguous() : weight;
-        b = bias.defined() ? bias.contiguous() : bias;
+        w = weight.defined() ? stored(weight).contiguous() : weight;
+        b = bias.defined() ? stored(bias).contiguous() : bias;
         y = at::empty_like(x);
         stats = at::empty({2 * samples * groups}, x.options().dtype(at::kFloat));
         ta_b200_group_norm_params p = group_norm_params(call, x, w, b, stats);
@@ -213,7 +223,7 @@ struct DropoutCall {
     bool last;                          // channels last in memory
 };
 
-Tensor in_order(const Tensor &t, bool last) { return last ? channels_last(t) : t.contiguous(); }
+Tensor in_order(const Tensor &t, bool last) { return last ? channels_last(t) : stored(t).contiguous(); }
 
 Tensor dropout_call(const DropoutCall &c, const Tensor &x, const Tensor &residual, const Tensor &seed)
 {
@@ -240,6 +250,7 @@ struct DropoutBackward : Node {
 
     variable_list apply(variable_list &&grads) override
     {
+        const std::lock_guard<std::mutex> lock(mutex_);        // two threads may go backward through one graph
         variable_list out(2);
         if (!grads[0].defined()) return out;
         if (task_should_compute_output(1)) out[1] = grads[0];
@@ -250,7 +261,11 @@ struct DropoutBackward : Node {
         }
         return once_differentiable(std::move(out), "dropout");
     }
-    void release_variables() override { seed.reset_data(); }
+    void release_variables() override
+    {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        seed.reset_data();
+    }
     std::string name() const override { return "TaDropoutBackward"; }
 };
 
@@ -265,7 +280,7 @@ Tensor dropout(const Tensor &x0, const optional<Tensor> &residual0, double p, ui
     Tensor y;
     {
         at::AutoGradMode off(false);
-        Tensor x = x0;
+        Tensor x = stored(x0);
         if (!x.is_contiguous()) {
             call.last = x.dim() >= 3 && x.dim() <= 5 && x.movedim(-3, -1).is_contiguous();
             if (!call.last) x = x.contiguous();
@@ -318,7 +333,7 @@ variable_list rotary_call(const RotaryCall &c, const Tensor &q, const Tensor &k,
     for (int which = 0; which < 2; ++which) {
         const Tensor &t = which ? k : q;
         if (!t.defined()) continue;
-        dense[which] = t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+        dense[which] = t.stride(-1) == 1 || t.size(-1) == 1 ? stored(t) : stored(t).contiguous();
         out[which] = at::empty_like(dense[which]);
         if (out[which].stride(-1) != 1 && t.size(-1) != 1)      // an expanded input: its copy is laid out by size
             out[which] = at::empty(t.sizes(), t.options());
@@ -340,6 +355,7 @@ struct RotaryBackward : Node {
 
     variable_list apply(variable_list &&grads) override
     {
+        const std::lock_guard<std::mutex> lock(mutex_);        // two threads may go backward through one graph
         variable_list out(2);
         const Tensor dq = task_should_compute_output(0) ? grads[0] : Tensor();
         const Tensor dk = grads.size() > 1 && task_should_compute_output(1) ? grads[1] : Tensor();
@@ -352,6 +368,7 @@ struct RotaryBackward : Node {
     }
     void release_variables() override
     {
+        const std::lock_guard<std::mutex> lock(mutex_);
         positions.reset_data();
         top.reset_data();
         left.reset_data();
@@ -381,7 +398,7 @@ py::capsule rotary_spec(std::vector<int> sections, int pairing, int spectrum, in
 py::object rotary(const Tensor &q, const optional<Tensor> &k0, const optional<Tensor> &positions0, const optional<Tensor> &top0, const optional<Tensor> &left0,
                   const optional<Tensor> &flip0, const py::capsule &spec)
 {
-    const Tensor k = given(k0), positions = given(positions0), top = given(top0), left = given(left0), flip = given(flip0);
+    const Tensor k = given(k0), positions = stored(given(positions0)), top = given(top0), left = given(left0), flip = given(flip0);
     const c10::cuda::OptionalCUDAGuard guard(q.device());
     const RotaryCall &call = *spec.get_pointer<RotaryCall>();
     const bool grad = wants_grad({&q, &k});
