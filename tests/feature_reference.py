@@ -158,8 +158,14 @@ def grid_positions(grid, n, patch=1.0, top=None, left=None, flip=None, device="c
 
 
 def assert_within(got, want, tol, what=""):
-    """Every element within its bound; NaN where NaN is expected."""
+    """Every element within its bound; NaN where NaN is expected.
+
+    A type rounds to infinity from half a step above its largest value M on.  The last step below M is
+    M eps / (2 - eps) (M = (2 - eps) 2^e, step eps 2^e), so that is M (1 + eps / (4 - 2 eps)): 65520 for float16.  Infinity
+    is right where the exact value and its bound reach that."""
+    top = torch.finfo(got.dtype).max * (1 + torch.finfo(got.dtype).eps / (4 - 2 * torch.finfo(got.dtype).eps))
     got, want = got.detach().double(), want.double()
     assert got.shape == want.shape, (what, tuple(got.shape), tuple(want.shape))
-    bad = ~((got - want).abs() <= tol) & ~((got == want) | (got.isnan() & want.isnan()))
+    over = got.isinf() & (got.sign() == want.sign()) & (want.abs() + tol >= top)
+    bad = ~((got - want).abs() <= tol) & ~((got == want) | (got.isnan() & want.isnan()) | over)
     assert not bool(bad.any()), (what, int(bad.sum()), float(((got - want).abs() / tol)[bad].max()), got[bad][:4].tolist(), want[bad][:4].tolist())

@@ -197,17 +197,66 @@ def test_captured_and_replayed_with_new_data():
             y = ta.group_norm(x, groups, w, b, activation="silu")
             outs = (y.detach(), *torch.autograd.grad(y, (x, w, b), dy))
         return graph, x, w, b, dy, outs
-    built = [build((2, 64, 40, 40), 8), build((3, 48, 21, 20), 4)]
+    built = [build((2, 64, 40, 40), 8), build((3, 33, 21, 20), 11), build((1, 128, 200, 200), 32)]     # clusters, odd channels, two launches
     for seed in (21, 22):
         for graph, x, w, b, dy, outs in built:
             with torch.no_grad():
                 x.copy_(_features(x.shape, x.dtype, seed))
             graph.replay()
         torch.cuda.synchronize()
-        for (graph, x, w, b, dy, outs), groups in zip(built, (8, 4)):
+        for (graph, x, w, b, dy, outs), groups in zip(built, (8, 11, 32)):
             want = R.group_norm(x.detach(), groups, w.detach(), b.detach(), 1e-5, "silu", dy=dy)
             for got, name in zip(outs, ("y", "dx", "dweight", "dbias")):
                 R.assert_within(got, want[name], want[name + "_tol"], name)
+
+
+@pytest.mark.parametrize("shape, groups", [((2, 40, 9, 9), 5), ((1, 40, 300, 200), 5)])
+def test_parameters_off_vector_boundaries(shape, groups):
+    """float32 weights that start in the middle of a vector, gradients included; 16-bit ones at odd elements."""
+    for dtype in TYPES:
+        pool = torch.randn(2, 41, device=DEV).to(dtype)
+        w, b = (pool[i, 1:].detach().requires_grad_() for i in (0, 1))
+        assert w.data_ptr() % 16 != 0
+        _check(_features(shape, torch.bfloat16).requires_grad_(), groups, w, b, "silu", dy=_features(shape, torch.bfloat16, 4))
+
+
+@pytest.mark.parametrize("side, rows, chain", [(30, 300, 20), (260, 133, 15)])
+def test_outliers_in_the_first_pixels(side, rows, chain):
+    """The eight pixels that a block takes its pivot from are d = 1000 spreads off.  Its `rows` rows add up to
+    rows d^2 where the deviations are 8 d^2, in chains of `chain` additions, each off by u: the squares' sum is off by
+    (chain + 3) u, the square of the sum by twice that, together 3 (chain + 3) rows / 8 u of the variance and half of it in
+    rstd; the mean by chain u d rows / side^2.  One cluster block of three, and one chunk of 512."""
+    x = _features((2, 32, side, side), torch.float32)[:2 if side == 30 else 1].contiguous(memory_format=torch.channels_last)
+    x[:, :, 0, :8] = 1000.0
+    w, b = _params(32, torch.float32)
+    y = ta.group_norm(x, 8, w, b)
+    want = R.group_norm(x, 8, w, b, 1e-5, "none")
+    total = side * side
+    spread = 1000.0 * (8 / total) ** 0.5                              # of the whole sample, to a per cent
+    xhat = ((want["y"] - b.double()[:, None, None]) / w.double()[:, None, None]).abs()
+    extra = R.U * (1.02 * 1.5 * (chain + 3) * rows / 8 * xhat + 1.02 * chain * 1000.0 / spread * rows / total)
+    R.assert_within(y, want["y"], want["y_tol"] + extra * w.double().abs()[:, None, None], "y")
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on the GPU share nothing: each gives the bits it gives alone."""
+    xs = [_features((4, 64, 64, 64), torch.bfloat16, s).requires_grad_() for s in (1, 2)]
+    dy = _features((4, 64, 64, 64), torch.bfloat16, 5)
+    alone = []
+    for x in xs:
+        y = ta.group_norm(x, 8, activation="silu")
+        alone.append((y.detach(), torch.autograd.grad(y, x, dy)[0]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(5):
+        got = []
+        for x, st in zip(xs, streams):
+            with torch.cuda.stream(st):
+                y = ta.group_norm(x, 8, activation="silu")
+                got.append((y.detach(), torch.autograd.grad(y, x, dy)[0]))
+        torch.cuda.synchronize()
+        for a, g in zip(alone, got):
+            assert torch.equal(a[0], g[0]) and torch.equal(a[1], g[1])
 
 
 def test_class_double_backward_and_scratch():

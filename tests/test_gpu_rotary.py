@@ -167,7 +167,7 @@ def test_rotation_is_undone_by_its_gradient():
     g, = torch.autograd.grad(ta.rotary_embedding(q, sections=(32, 32), grid=(3, 4)), q, dy)
     f = lambda t: ta.rotary_embedding(t.detach(), sections=(32, 32), grid=(3, 4)).double()
     num, ana = float(((f(q + d) - f(q)) * dy.double()).sum()), float((g.double() * d.double()).sum())
-    assert abs(num - ana) <= 64 * R.U * float(((q.abs() + d.abs()) * dy.abs()).double().sum()) * 2
+    assert abs(num - ana) <= 64 * R.U * float(((q.detach().abs() + d.abs()) * dy.abs()).double().sum()) * 2
 
 
 def test_captured_single_tokens():

@@ -7,7 +7,6 @@
 #include "ta_features.h"
 #include "ta_pack.cuh"
 
-
 namespace ta {
 
 // ----------------------------------------------------------------------------- activations
@@ -17,19 +16,11 @@ __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.f
 __device__ __forceinline__ float rcp_fast(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 constexpr float kLog2E = 1.4426950408889634f;
 
-// 1 / (1 + e^-z).  (One reciprocal for two values, 1 / (d0 d1) times the other factor, would spare the special
-// function unit a quarter of its work, but costs eight more instructions per pair: these kernels wait for
-// instruction issue first.)
+// 1 / (1 + e^-z).  (One reciprocal for two values, 1 / (d0 d1) times the other factor, is worth 2 % forward and costs 1 %
+// backward: 4 x 128 x 224^2 bfloat16 36.5 -> 35.5 us, 64 x 320 x 28^2 bfloat16 backward 49.5 -> 50.1 us.  The product needs
+// e^-z held to 2^60, so that results below z = -41 are wrong by orders of magnitude: not taken.)
 template <bool FAST> __device__ __forceinline__ float2 sigmoid2(float2 z)
 {
-#ifdef GN_PAIR
-    if constexpr (FAST) {
-    const float2 e = mul2(z, both(-kLog2E));
-    const float2 d = add2(make_float2(exp2_fast(fminf(e.x, 60.0f)), exp2_fast(fminf(e.y, 60.0f))), both(1.0f));
-    const float r = rcp_fast(d.x * d.y);
-    return make_float2(r * d.y, r * d.x);
-    }
-#endif
     if constexpr (!FAST) return make_float2(1.0f / (1.0f + expf(-z.x)), 1.0f / (1.0f + expf(-z.y)));
     const float2 e = mul2(z, both(-kLog2E)), d = add2(make_float2(exp2_fast(e.x), exp2_fast(e.y)), both(1.0f));
     return make_float2(rcp_fast(d.x), rcp_fast(d.y));
@@ -212,12 +203,16 @@ __device__ __forceinline__ float2 group_sum(const GnLanes &l, const float2 *red,
 // Two launches a pass: the first reduces chunks of rows, the second reads the same rows again, last ones first
 // since those are still in the L2 cache, and writes the result.  (Ranges of samples that fit the cache, one pair
 // of launches each, were slower for all that the gaps between launches cost: 16 x 128 x 224^2 float16 in
-// 64 MB ranges 162 us, in one pair 116 us.)
+// 64 MB ranges 162 us against 116 in one pair, both with rows held in registers.)
 //
 // A block covers a tile of channel vectors and a chunk of rows; thread t holds vector t % tile of rows
 // t / tile + i rows_per_step.  Tiles hold whole groups (groups_per_tile); a group wider than a block is
 // cut into `split` tiles.  Each block leaves one partial result per group of its tile:
 // part[((n groups + g) chunks + chunk) split + piece].
+//
+// What bounds it: the memory for large tensors, three passes over the features forward and five backward
+// (16 x 128 x 224^2 float16 with SiLU, 617 MB, 111 us = 5.5 TB/s); instruction issue where the second pass reads the L2 cache
+// (4 x 128 x 224^2 bfloat16 36 us forward, 61 us backward).  Rows held in registers instead of the ring: 122, 44, 73 us.
 constexpr int kGnThreads = 256;
 constexpr int kGnBlocksForward = 4, kGnBlocksBackward = 3;       // blocks per SM (64 and 80 registers a thread)
 struct GnShape {
@@ -407,19 +402,12 @@ __device__ __forceinline__ float2 moments_of(float pivot, float2 t, float inv)
     const float q = fmaf(-t.x * inv, t.x, t.y);
     return make_float2(fmaf(t.x, inv, pivot), q < 0.0f ? 0.0f : q);       // (a NaN stays)
 }
-template <int P, typename Vec> __device__ __forceinline__ void add_values(const Vec &p, float2 (&sm)[P])
-{
-    float2 f[P];
-    p.unpack(f);
-#pragma unroll
-    for (int j = 0; j < P; ++j) sm[j] = add2(sm[j], f[j]);
-}
-
 // Per (sample, group, chunk): mean and sum of squared deviations from it.
 //
-// The pivot of a group: the mean of its first channel in the block's first rows, up to eight.  Sums of differences to it
-// and of their squares lose count / 8 x 2^-24 of the variance at the very worst (a pivot made of the group's only
-// outlier), as a rule a few 2^-24, however far from zero the values lie.
+// The pivot of a group: the mean of its first channel in the block's first rows, up to eight.  However far from zero the
+// values lie, the sums of differences to it and of their squares lose a few 2^-24 of the variance as a rule.  At the very
+// worst, a pivot made of nothing but outliers d away from the block's other rows, the squares add up to rows x d^2 where
+// their deviations are 8 d^2: chains of L additions then lose up to 3 (L + 3) rows / 8 x 2^-24 of the block's variance.
 template <typename T, int V>
 __global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_stats_kernel(const __grid_constant__ GnArgs a, const __grid_constant__ GnShape s)
 {

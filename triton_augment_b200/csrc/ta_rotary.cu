@@ -107,6 +107,9 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_scalar_kernel(const __g
 }
 
 // ----------------------------------------------------------------------------- vector kernel
+// Bound by the memory: 16 x 4096 tokens x 32 heads x 128 bfloat16 (1.07 GB) 181 us in halves, 177 us interleaved = 91, 93 % of the
+// copy bandwidth; 8 x 1568 tokens x 24 heads x 64 (77 MB) 20 us = 59 %; single tokens 3.7 us, latency.
+//
 // A thread owns one vector of a token's head (two, half the rotated part apart, with HALVES), computes the
 // cosines and sines of its pairs once and turns that vector in every `head_step`-th head of q and k,
 // kRotaryBatch heads' loads in flight.  A block covers `block_units` of the head's vectors x head_step heads x
