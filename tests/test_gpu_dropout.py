@@ -85,6 +85,28 @@ def test_shared_masks(shape, mode, same_on_batch, same_on_frame, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("same_on_batch, same_on_frame", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("shape, mode, last", [
+    ((2, 3, 64, 70), "channel", True), ((3, 33, 40, 41), "channel", True), ((2, 2, 63, 67), "channel", True), ((2, 256, 5, 7), "channel", True),
+    ((2, 4096, 1, 2), "channel", True), ((2, 4097, 1, 2), "channel", True), ((3, 2047, 1, 5), "channel", True), ((2, 3, 5, 50, 60), "channel", True),
+    ((2, 1, 1, 4096), "channel", True), ((3, 31, 17, 16), "pixel", False), ((2, 6, 3, 30, 31), "pixel", False), ((2, 9, 5, 11, 19), "element", False),
+    ((3, 4, 9, 17, 15), "element", True)])
+def test_masks_that_repeat(shape, mode, last, same_on_batch, same_on_frame, dtype):
+    """A row of entries shared by the rows above it: short and long rows, planes that end inside a vector and inside a block."""
+    shared = _shared(len(shape), mode, same_on_batch, same_on_frame)
+    x, nd = _randn(shape, dtype), len(shape)
+    r = _randn(shape, dtype, 1)
+    order = list(range(nd - 3)) + [nd - 2, nd - 1, nd - 3] if last else None
+    if last:
+        x = x.movedim(-3, -1).contiguous().movedim(-1, -3)
+        if x.is_contiguous():
+            order = None
+    for residual in (None, r):
+        _check(x, 0.4, 5, residual=residual, shared=shared, order=order, mode=mode, same_on_batch=same_on_batch, same_on_frame=same_on_frame)
+    assert not bool(ta.dropout(x, 1.0, 5, mode=mode, same_on_batch=same_on_batch, same_on_frame=same_on_frame).any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("mode", ["element", "channel"])
 def test_gradients(mode, dtype):
     """dx = keep dy / (1 - p), the residual's gradient is dy itself."""

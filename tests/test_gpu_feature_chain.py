@@ -57,7 +57,7 @@ def test_block_against_64_bits():
     leaves64 = [t.detach().double().requires_grad_() for t in leaves]
     loss64, q64 = _block(images, *leaves64, top, left, flip, (gn64, drop64, rope64))
     grads64 = torch.autograd.grad(loss64, leaves64)
-    assert abs(float(loss - loss64)) <= 1e-4 * abs(float(loss64))
+    assert abs(float((loss - loss64).detach())) <= 1e-4 * abs(float(loss64))
     assert float((q - q64).abs().max()) <= 1e-4 * float(q64.abs().max())
     for got, want in zip(grads, grads64):
         assert float((got - want).norm()) <= 1e-3 * float(want.norm())
