@@ -45,7 +45,7 @@ def _check(x, groups, weight, bias, act, eps=1e-5, same_on_frame=False, dy=None)
 # one pixel to many, odd planes, groups of one channel to all, channel counts of every vector width
 SHAPES = [((1, 8, 1, 1), 2), ((1, 64, 14, 14), 8), ((3, 320, 9, 7), 32), ((2, 30, 17, 5), 6), ((2, 33, 5, 6), 11), ((5, 7, 3, 3), 7),
           ((2, 36, 31, 2), 4), ((1, 16, 1, 257), 1), ((2, 1, 40, 40), 1), ((1, 2056, 3, 3), 8), ((4, 512, 1, 1), 32), ((2, 96, 65, 67), 12),
-          ((1, 130, 64, 48), 10), ((70, 16, 5, 5), 4), ((2, 40, 128, 130), 4)]
+          ((1, 130, 64, 48), 10), ((70, 16, 5, 5), 4), ((2, 40, 128, 130), 4), ((3, 320, 14, 14), 32), ((2, 640, 14, 13), 32)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

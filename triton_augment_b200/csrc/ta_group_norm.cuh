@@ -4,6 +4,8 @@
 //   sample's group.  With g = dy * act'(z) and u = g * weight:
 //   dweight = sum g * xhat, dbias = sum g, dx = rstd * (u - mean(u) - xhat * mean(u * xhat)).
 #pragma once
+#include <atomic>
+
 #include "ta_features.h"
 #include "ta_pack.cuh"
 
@@ -121,6 +123,16 @@ template <int V, typename Get> __device__ __forceinline__ void spread_groups(int
         for (int i = 0; i < (V + 1) / 2; ++i) { x[i] = both(t.x); y[i] = both(t.y); }
         return;
     }
+    if (V >= 4 && cpg >= V) {                             // two groups, and the threads of a warp cut at different places: selected
+        const float2 next = get(group + 1);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float2 s = j < left ? t : next;
+            if (j % 2) { x[j / 2].y = s.x; y[j / 2].y = s.y; }
+            else { x[j / 2].x = s.x; y[j / 2].x = s.y; }
+        }
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         if (left == 0) { t = get(++group); left = cpg; }
@@ -144,16 +156,18 @@ template <int V> __device__ __forceinline__ void store_folded(float2 *dst, const
 #pragma unroll
             for (int i = 0; i < V; i += 2 * w) s[i] = add2(s[i], s[i + w]);
         }
-    if (fold == V) { dst[0] = s[0]; return; }
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (i % fold == 0) dst[i / fold] = s[i];
+    for (int w = 1; w <= V; w *= 2)                       // (constants: a division by `fold` costs more than all else here)
+        if (w == fold) {
+#pragma unroll
+            for (int i = 0; i < V; i += w) dst[i / w] = s[i];
+        }
 }
 
 // How a block adds up its groups: `lanes` lanes each, the same order every time.  A group's entries are
 // `width` neighbouring values in each of a number of rows.
 struct GnLanes {
-    int lanes, width, row_step, entry_step;              // a lane's next entry: row_step rows and entry_step values on
+    int lanes, shift, per_pass, width, row_step, entry_step;      // lanes = 1 << shift, groups of a pass; a lane's next entry: row_step rows and entry_step values on
     FastDiv width_div;
 };
 __host__ inline GnLanes gn_lanes(int groups, int threads, int width)
@@ -161,6 +175,9 @@ __host__ inline GnLanes gn_lanes(int groups, int threads, int width)
     GnLanes l;
     l.lanes = 32;
     while (l.lanes > 1 && groups * l.lanes > threads) l.lanes >>= 1;
+    l.shift = 0;
+    while ((1 << l.shift) < l.lanes) ++l.shift;
+    l.per_pass = threads >> l.shift;
     l.width = width;
     l.row_step = l.lanes / width;
     l.entry_step = l.lanes % width;
@@ -212,14 +229,14 @@ __device__ __forceinline__ float2 group_sum(const GnLanes &l, const float2 *red,
 //
 // What bounds it: the memory for large tensors, three passes over the features forward and five backward
 // (16 x 128 x 224^2 float16 with SiLU, 617 MB, 111 us = 5.5 TB/s); instruction issue where the second pass reads the L2 cache
-// (4 x 128 x 224^2 bfloat16 36 us forward, 61 us backward).  Rows held in registers instead of the ring: 122, 44, 73 us.
+// (4 x 128 x 224^2 bfloat16 36 us forward, 60 us backward).  Rows held in registers instead of the ring: 122, 44, 73 us.
 constexpr int kGnThreads = 256;
 constexpr int kGnBlocksForward = 4, kGnBlocksBackward = 3;       // blocks per SM (64 and 80 registers a thread)
 struct GnShape {
-    int vecs, tile, tiles, rows_per_step, groups_per_tile, split, unit, chunks, fold;
+    int vecs, tile, tiles, rows_per_step, groups_per_tile, split, unit, chunks, fold, per_vec;      // per_vec: folded values of a vector
+    float inv;                          // 1 / (values of a group in the sample)
     long long chunk_rows;
     GnLanes columns;                    // sums over a tile's columns
-    int finish_lanes;                   // lanes a group's chunks are joined by
 };
 
 __host__ __device__ inline int gn_gcd(int a, int b) { while (b) { const int t = a % b; a = b; b = t; } return a; }
@@ -249,7 +266,8 @@ __host__ inline GnShape gn_shape(const GnArgs &a, int v, bool backward)
     s.fold = v;
     while (a.cpg % s.fold) s.fold /= 2;
     s.columns = gn_lanes(s.groups_per_tile, kGnThreads, (s.split == 1 ? a.cpg : s.tile * v) / s.fold);
-    s.finish_lanes = s.columns.lanes;
+    s.per_vec = v / s.fold;
+    s.inv = 1.0f / ((float)a.rows * (float)a.cpg);
     // one wave of blocks where the samples allow it, at least four steps a thread
     const long long want = (long long)(backward ? kGnBlocksBackward : kGnBlocksForward) * a.sm_count / (a.n * s.tiles);
     const long long most = (a.rows + 4LL * s.rows_per_step - 1) / (4LL * s.rows_per_step);
@@ -419,7 +437,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_stats_kernel(
     GnStream<T, V, 1, kGnAhead> rows;
     rows.src[0] = (const T *)a.x + (at.n * a.rows + at.row0 + at.r) * a.channels + at.vec * V;
     rows.start(smem, (long long)s.rows_per_step * a.channels, count);
-    const int per_vec = V / s.fold, stride = s.tile * per_vec, groups = at.groups(a, s);
+    const int per_vec = s.per_vec, stride = s.tile * per_vec, groups = at.groups(a, s);
     const int width = s.split == 1 ? s.columns.width : at.width(s) * per_vec;
     const int sample_rows = min(min(8, s.rows_per_step), at.rows);
     const float sample_inv = 1.0f / (float)sample_rows;
@@ -436,7 +454,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_stats_kernel(
     __syncthreads();
     const int group = at.active ? (at.vec * V) / a.cpg - at.group0 : 0;
     spread_groups<V>(group, at.active ? a.cpg - (at.vec * V) % a.cpg : V, a.cpg, [&](int g) { return make_float2(-pivot_of(g), 0.0f); }, pv, sm);
-    const int lanes = s.columns.lanes, per_pass = kGnThreads / lanes, lane = threadIdx.x & (lanes - 1), mine = threadIdx.x / (unsigned)lanes;
+    const int lanes = s.columns.lanes, per_pass = s.columns.per_pass, lane = threadIdx.x & (lanes - 1), mine = threadIdx.x >> s.columns.shift;
     constexpr int kSums = kGnThreads * V * (int)sizeof(float2), kRing = GnStream<T, V, 1, kGnAhead>::kBytes;
     float *pivots = reinterpret_cast<float *>(smem + (kRing > kSums ? kRing : kSums));          // [groups]
     for (int g = threadIdx.x; g < groups; g += kGnThreads) pivots[g] = pivot_of(g);
@@ -460,15 +478,15 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_stats_kernel(
 // Mean and rstd of the tile's groups from their chunks, into stat[]
 __device__ __forceinline__ void gn_finish_stats(const GnArgs &a, const GnShape &s, const GnPlace &at, int v, float2 *stat)
 {
-    const int groups = at.groups(a, s), lanes = s.finish_lanes, lane = threadIdx.x & (lanes - 1), entries = s.chunks * s.split;
-    const float inv = 1.0f / ((float)a.rows * (float)a.cpg);
+    const int groups = at.groups(a, s), lanes = s.columns.lanes, lane = threadIdx.x & (lanes - 1), entries = s.chunks * s.split;
+    const float inv = s.inv;
     const auto values = [&](int e) {
         if (s.split == 1) return (float)min(s.chunk_rows, a.rows - e * s.chunk_rows) * (float)a.cpg;
         const int chunk = e / s.split;
         return (float)min(s.chunk_rows, a.rows - chunk * s.chunk_rows) * (float)(min(s.tile, s.unit - (e - chunk * s.split) * s.tile) * v);
     };
-    for (int base = 0; base < groups; base += kGnThreads / lanes) {
-        const int g = base + threadIdx.x / lanes;
+    for (int base = 0; base < groups; base += s.columns.per_pass) {
+        const int g = base + (threadIdx.x >> s.columns.shift);
         const bool valid = g < groups;
         const long long id = (long long)at.n * a.groups + at.group0 + g;
         const float2 *part = a.part + id * entries;
@@ -541,10 +559,10 @@ __host__ __device__ inline float2 *gn_channel_part(const GnArgs &a, const GnShap
 // and then the parts are added.  Ends with the block synchronised.
 __device__ __forceinline__ void sum_columns(float2 *acc, int stride, int columns, int rows, int threads)
 {
-    int parts = threads / columns;
-    parts = parts < 1 ? 1 : parts > rows ? rows : parts;
+    int parts = 2 * columns > threads ? 1 : threads / columns;
+    parts = parts > rows ? rows : parts;
     for (int i = threadIdx.x; i < columns * parts; i += threads) {
-        const int part = i / columns, c = i - part * columns;
+        const int part = parts == 1 ? 0 : i / columns, c = i - part * columns;
         float2 t = acc[part * stride + c];
 #pragma unroll 4
         for (int k = part + parts; k < rows; k += parts) { const float2 e = acc[k * stride + c]; t = add2(t, e); }
@@ -598,7 +616,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_sums_ke
         });
         __syncthreads();
         // sums of (u xhat, rstd u) of the groups: u xhat = g scale (x - mean)
-        const int per_vec = V / s.fold, stride = s.tile * per_vec, groups = at.groups(a, s), lanes = s.columns.lanes, lane = threadIdx.x & (lanes - 1);
+        const int per_vec = s.per_vec, stride = s.tile * per_vec, groups = at.groups(a, s), lanes = s.columns.lanes, lane = threadIdx.x & (lanes - 1);
         const int width = s.split == 1 ? s.columns.width : at.width(s) * per_vec;
         if (at.r < s.rows_per_step) {
             float2 ux[P], u[P];
@@ -607,8 +625,8 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_sums_ke
             store_folded<V>(acc + at.r * stride + at.v * per_vec, ux, u, s.fold);
         }
         __syncthreads();
-        for (int base = 0; base < groups; base += kGnThreads / lanes) {
-            const int g = base + threadIdx.x / (unsigned)lanes;
+        for (int base = 0; base < groups; base += s.columns.per_pass) {
+            const int g = base + (threadIdx.x >> s.columns.shift);
             const float2 t = group_sum(s.columns, acc, stride, s.rows_per_step, width, g, g < groups);
             if (g < groups && lane == 0)
                 a.part[(((long long)at.n * a.groups + at.group0 + g) * s.chunks + at.chunk) * s.split + at.piece] = t;
@@ -685,10 +703,10 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_input_k
 #pragma unroll
     for (int j = 0; j < P; ++j) scale[j] = mul2(scale[j], rstd[j]);
     gn_wait_first();
-    const int groups = at.groups(a, s), lanes = s.finish_lanes, lane = threadIdx.x & (lanes - 1), entries = s.chunks * s.split;
-    const float inv = 1.0f / ((float)a.rows * (float)a.cpg);
-    for (int base = 0; base < groups; base += kGnThreads / lanes) {
-        const int g = base + threadIdx.x / lanes;
+    const int groups = at.groups(a, s), lanes = s.columns.lanes, lane = threadIdx.x & (lanes - 1), entries = s.chunks * s.split;
+    const float inv = s.inv;
+    for (int base = 0; base < groups; base += s.columns.per_pass) {
+        const int g = base + (threadIdx.x >> s.columns.shift);
         float ux = 0.0f, u = 0.0f;
         if (g < groups) {
             const float2 *part = a.part + ((long long)at.n * a.groups + at.group0 + g) * entries;
@@ -722,6 +740,20 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_input_k
 }
 
 // ----------------------------------------------------------------------------- launches
+// Shared memory and cluster sizes beyond the defaults, once per device (twice does no harm)
+template <auto kernel, bool CLUSTER> cudaError_t gn_prepare(int bytes)
+{
+    static std::atomic<unsigned> ready{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    if (device < 32 && (ready.load(std::memory_order_acquire) >> device) & 1u) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && CLUSTER) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && device < 32) ready.fetch_or(1u << device, std::memory_order_release);
+    return e;
+}
+
 template <typename Kernel, typename... Args>
 cudaError_t gn_launch_kernel(Kernel kernel, dim3 grid, size_t smem, bool dependent, cudaStream_t stream, Args... args)
 {
@@ -767,8 +799,16 @@ template <typename T, int V> cudaError_t gn_launch_streaming(const GnArgs &all, 
         return e != cudaSuccess ? e : gn_launch_kernel(gn_apply_kernel<T, V>, grid, ring + stat, true, stream, a, s);
     }
     a.channel_part = gn_channel_part(a, s);
-    e = gn_launch_kernel(gn_grad_sums_kernel<T, V>, grid, grad_ring > sums ? grad_ring : sums, false, stream, a, s);
-    if (e == cudaSuccess && a.dx) e = gn_launch_kernel(gn_grad_input_kernel<T, V>, grid, grad_ring + stat, true, stream, a, s);
+    // A quarter of an SM's shared memory keeps a fourth block off it: kernels with narrow vectors need so few registers that
+    // the second launch's blocks would crowd on the SMs that are free first (32 x 33 x 112^2 float32 132 us against 104,
+    // 16 x 130 x 96^2 bfloat16 81 against 67; forward, where up to four blocks fit, no difference).
+    // (A tile has kGnThreads V channels at most, and no more groups.)
+    constexpr int grad_bytes = 57 * 1024;
+    static_assert(kGnBlocksBackward == 3 && grad_ring + kGnThreads * V * sizeof(float2) <= grad_bytes);
+    e = gn_prepare<gn_grad_sums_kernel<T, V>, false>(grad_bytes);
+    if (e == cudaSuccess) e = gn_launch_kernel(gn_grad_sums_kernel<T, V>, grid, grad_bytes, false, stream, a, s);
+    if (e == cudaSuccess && a.dx) e = gn_prepare<gn_grad_input_kernel<T, V>, false>(grad_bytes);
+    if (e == cudaSuccess && a.dx) e = gn_launch_kernel(gn_grad_input_kernel<T, V>, grid, grad_bytes, true, stream, a, s);
     if (e == cudaSuccess && (a.dweight || a.dbias)) e = gn_launch_params(a, a.channel_part, a.n * s.chunks, stream);
     return e;
 }

@@ -7,11 +7,13 @@
 // the copies.  The share is loaded in four parts and added up part by part as they arrive.
 //
 // What bounds it: the time a block lives, of which the copies take a third and the arithmetic another; about 200 KB
-// per SM are in flight.  32 x 256 x 56^2 bfloat16 with SiLU 32.5 us forward, 61.4 us backward; 64 x 320 x 28^2 27.8 and 49.5 us.
+// per SM are in flight.  32 x 256 x 56^2 bfloat16 with SiLU 32.2 us forward, 60.5 us backward; 64 x 320 x 28^2 25.7 and 45.9 us.
+// (Divisions by powers of two known on the host, and groups looked up in branches, had made those 27.9 and 49.3 us.)
 // (Clusters that stay and fetch the next sample into a second buffer meanwhile have half the blocks
-// per SM to hide the latency of the sums: 32 x 256 x 56^2 bfloat16 37 us against 34, both before the pivot's one reduction.)
+// per SM to hide the latency of the sums: 32 x 256 x 56^2 bfloat16 37 us against 34, both before the pivot's one reduction.
+// Clusters that start up to 3 us apart, so that copies and arithmetic of different ones overlap: 3 % faster there, 2 % slower
+// on 64 x 320 x 28^2, 14 % on 64 x 1024 x 7^2.)
 #pragma once
-#include <atomic>
 
 namespace ta {
 
@@ -27,7 +29,8 @@ __device__ __forceinline__ void copy_wait(int left)
 // A cluster of `ranks` blocks covers a slab of `vecs` channel vectors; block k holds rows [k rows_per_block, ...),
 // thread t channel vector t % vecs of rows t / vecs + i rows_per_step, i < steps.
 struct GnPlan {
-    int threads, ranks, vecs, slabs, rows_per_step, groups, fold, steps, smem, rows_per_block;
+    int threads, ranks, vecs, slabs, rows_per_step, groups, fold, per_vec, steps, smem, rows_per_block;      // per_vec: folded values of a vector
+    float inv, block_inv;               // 1 / (values of a group in the sample), in a full block
     int data_bytes;                     // of the features, in front of everything else in shared memory
     FastDiv vecs_div, step_div, cpg_div, slab_div;
     GnLanes columns;                    // sums over the slab's columns
@@ -69,7 +72,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_kernel(const __gri
 {
     constexpr int V = 16 / sizeof(T), P = V / 2;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int slots = p.rows_per_step * p.vecs, per_vec = V / p.fold, stride = p.vecs * per_vec;
+    const int slots = p.rows_per_step * p.vecs, per_vec = p.per_vec, stride = p.vecs * per_vec;
     Pack<T, V> *data = reinterpret_cast<Pack<T, V> *>(smem) + threadIdx.x;             // [steps][slots]
     float2 *pub = reinterpret_cast<float2 *>(smem + p.data_bytes);                     // [groups] this block's (mean, squared deviations), read by the cluster
     float2 *stat = pub + p.groups;                      // [groups] the sample's (mean, rstd)
@@ -92,7 +95,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_kernel(const __gri
     // The pivot of a group: the mean of its first channel over the block's first rows, up to eight, with the loss
     // that gn_stats_kernel states.
     const int sample_rows = min(min(8, p.rows_per_step), at.rows);
-    const float sample_inv = sample_rows > 0 ? 1.0f / (float)sample_rows : 0.0f;
+    const float sample_inv = sample_rows == 8 ? 0.125f : sample_rows > 0 ? 1.0f / (float)sample_rows : 0.0f;
     const auto pivot_of = [&](int g) {
         const T *first = reinterpret_cast<const T *>(smem) + g * a.cpg;
         float s = 0.0f;
@@ -114,8 +117,8 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_kernel(const __gri
         for (int i = q * quarter; i < end; ++i) add_moments<P>(data[i * slots], pv, sm, s2);
     }
     if (at.holds) store_folded<V>(red + at.r * stride + at.v * per_vec, sm, s2, p.fold);
-    const int lanes = p.columns.lanes, lane = threadIdx.x & (lanes - 1), per_pass = THREADS / lanes, mine = threadIdx.x / (unsigned)lanes;
-    const float block_inv = 1.0f / ((float)max(at.rows, 1) * (float)a.cpg), inv = 1.0f / ((float)a.rows * (float)a.cpg);
+    const int lanes = p.columns.lanes, lane = threadIdx.x & (lanes - 1), per_pass = p.columns.per_pass, mine = threadIdx.x >> p.columns.shift;
+    const float block_inv = at.rows == p.rows_per_block ? p.block_inv : 1.0f / ((float)max(at.rows, 1) * (float)a.cpg);
     const float full = (float)p.rows_per_block * (float)a.cpg;
     const auto values = [&](int k) { return k < p.ranks - 1 && (k + 1) * p.rows_per_block <= (int)a.rows ? full : (float)max(0, min(p.rows_per_block, (int)a.rows - k * p.rows_per_block)) * (float)a.cpg; };
     __syncthreads();
@@ -145,8 +148,8 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_kernel(const __gri
         }
         t = lane_sum(t, lanes);
         if (valid && lane == 0) {
-            const float2 m = moments_of(ref, t, inv);
-            const float rstd = rsqrtf(m.y * inv + a.eps);
+            const float2 m = moments_of(ref, t, p.inv);
+            const float rstd = rsqrtf(m.y * p.inv + a.eps);
             stat[g] = make_float2(m.x, rstd);
             if (at.rank == 0) {
                 const long long id = (long long)at.n * a.groups + at.slab * p.groups + g;
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_grad_kernel(const 
 {
     constexpr int V = 16 / sizeof(T), P = V / 2;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int slots = p.rows_per_step * p.vecs, columns = p.vecs * V, per_vec = V / p.fold, stride = p.vecs * per_vec;
+    const int slots = p.rows_per_step * p.vecs, columns = p.vecs * V, per_vec = p.per_vec, stride = p.vecs * per_vec;
     Pack<T, V> *xs = reinterpret_cast<Pack<T, V> *>(smem) + threadIdx.x, *ds = xs + (size_t)p.steps * slots;      // [steps][slots] each
     float2 *pub = reinterpret_cast<float2 *>(smem + p.data_bytes);                     // [groups] sums of (u xhat, rstd u), read by the cluster
     float2 *stat = pub + p.groups;                      // [groups] the sample's means of (u xhat, rstd u)
@@ -237,21 +240,20 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_grad_kernel(const 
         store_folded<V>(red + at.r * stride + at.v * per_vec, ux, u, p.fold);
     }
     __syncthreads();
-    for (int base = 0; base < at.groups; base += THREADS / lanes) {
-        const int g = base + threadIdx.x / (unsigned)lanes;
+    for (int base = 0; base < at.groups; base += p.columns.per_pass) {
+        const int g = base + (threadIdx.x >> p.columns.shift);
         const float2 t = group_sum(p.columns, red, stride, p.rows_per_step, p.columns.width, g, g < at.groups);
         if (g < at.groups && lane == 0) pub[g] = t;
     }
     if (p.ranks > 1) { cluster_arrive(); cluster_wait(); }
     else __syncthreads();
-    const float inv = 1.0f / ((float)a.rows * (float)a.cpg);
-    for (int base = 0; base < at.groups; base += THREADS / lanes) {
-        const int g = base + threadIdx.x / (unsigned)lanes;
+    for (int base = 0; base < at.groups; base += p.columns.per_pass) {
+        const int g = base + (threadIdx.x >> p.columns.shift);
         float2 t = make_float2(0.0f, 0.0f);
         if (g < at.groups)
             for (int k = lane; k < p.ranks; k += lanes) t = add2(t, p.ranks > 1 ? load_rank(pub + g, k) : pub[g]);
         t = lane_sum(t, lanes);
-        if (g < at.groups && lane == 0) stat[g] = make_float2(t.x * inv, t.y * inv);
+        if (g < at.groups && lane == 0) stat[g] = make_float2(t.x * p.inv, t.y * p.inv);
     }
     if (p.ranks > 1) cluster_arrive();                  // done with the others' memory
     __syncthreads();
@@ -296,20 +298,6 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_grad_kernel(const 
 }
 
 // ----------------------------------------------------------------------------- choice of the plan
-// Shared memory and cluster size beyond the defaults, once per device (twice does no harm)
-template <auto kernel> cudaError_t gn_prepare_cluster()
-{
-    static std::atomic<unsigned> ready{0};
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess) return e;
-    if (device < 32 && (ready.load(std::memory_order_acquire) >> device) & 1u) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess && device < 32) ready.fetch_or(1u << device, std::memory_order_release);
-    return e;
-}
-
 // false: a slab of whole groups does not fit a cluster's shared memory
 template <typename T> bool gn_plan(const GnArgs &a, int v, bool backward, GnPlan &p)
 {
@@ -323,7 +311,10 @@ template <typename T> bool gn_plan(const GnArgs &a, int v, bool backward, GnPlan
         for (int i = 0; i < 3; ++i)
             for (int seg = all < 32 ? all : 32; seg >= 1; seg = seg == 1 ? 0 : (seg + 1) / 2) {
                 const Class &c = backward ? backward_classes[i] : forward_classes[i];
-                const int vecs = (seg + unit - 1) / unit * unit;
+                // slabs of whole units, alike but for one unit: 40 vectors in units of 5 are 20 + 20, not 35 + 5 (half the
+                // blocks would hold next to nothing: 256 x 320 x 14^2 bfloat16 40.4 us against 26.9, backward 78 against 50)
+                const int units = all / unit, most_units = (seg + unit - 1) / unit, slabs = (units + most_units - 1) / most_units;
+                const int vecs = (units + slabs - 1) / slabs * unit;
                 if (vecs * 16 < 64 && vecs < all) break;                // row segments of at least 64 bytes (32: 187 us against 122 on 16 x 128 x 224^2)
                 if (vecs > c.threads) continue;
                 p.threads = c.threads;
@@ -349,6 +340,9 @@ template <typename T> bool gn_plan(const GnArgs &a, int v, bool backward, GnPlan
                 p.step_div = fast_div_of(p.rows_per_step);
                 p.cpg_div = fast_div_of(a.cpg);
                 p.slab_div = fast_div_of(p.slabs);
+                p.per_vec = v / p.fold;
+                p.inv = 1.0f / ((float)a.rows * (float)a.cpg);
+                p.block_inv = 1.0f / ((float)p.rows_per_block * (float)a.cpg);
                 p.columns = gn_lanes(p.groups, p.threads, a.cpg / p.fold);
                 return p.smem <= c.bytes && a.n * p.slabs * ranks < (1LL << 31);
             }
@@ -358,7 +352,7 @@ template <typename T> bool gn_plan(const GnArgs &a, int v, bool backward, GnPlan
 template <auto kernel, typename... Args>
 cudaError_t gn_launch_cluster(const GnPlan &p, long long samples, cudaStream_t stream, Args... args)
 {
-    const cudaError_t e = gn_prepare_cluster<kernel>();
+    const cudaError_t e = gn_prepare<kernel, true>(113 * 1024);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(samples * p.slabs * p.ranks));
