@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_kernel(const __gri
 template <typename T, int THREADS, int PER_SM>
 __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_grad_kernel(const __grid_constant__ GnArgs a, const __grid_constant__ GnPlan p, float2 *channel_sums)
 {
+    gn_allow_second();                                  // the parameters' gradients
     constexpr int V = 16 / sizeof(T), P = V / 2;
     extern __shared__ __align__(16) unsigned char smem[];
     const int slots = p.rows_per_step * p.vecs, columns = p.vecs * V, per_vec = p.per_vec, stride = p.vecs * per_vec;
