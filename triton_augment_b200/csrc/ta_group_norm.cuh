@@ -229,7 +229,7 @@ __device__ __forceinline__ float2 group_sum(const GnLanes &l, const float2 *red,
 //
 // What bounds it: the memory for large tensors, three passes over the features forward and five backward
 // (16 x 128 x 224^2 float16 with SiLU, 617 MB, 111 us = 5.5 TB/s); instruction issue where the second pass reads the L2 cache
-// (4 x 128 x 224^2 bfloat16 36 us forward, 60 us backward).  Rows held in registers instead of the ring: 122, 44, 73 us.
+// (4 x 128 x 224^2 bfloat16 35 us forward, 58 us backward).  Rows held in registers instead of the ring: 122, 44, 73 us.
 constexpr int kGnThreads = 256;
 constexpr int kGnBlocksForward = 4, kGnBlocksBackward = 3;       // blocks per SM (64 and 80 registers a thread)
 struct GnShape {
@@ -406,12 +406,11 @@ constexpr int kGnAhead = 8, kGnAheadGrad = 4;
 template <int P, typename Vec> __device__ __forceinline__ void add_moments(const Vec &p, const float2 (&pv)[P], float2 (&sm)[P], float2 (&s2)[P])
 {
     float2 f[P];
-    p.unpack(f);
+    p.unpack_plus(pv, f);
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-        const float2 d = add2(f[j], pv[j]);
-        sm[j] = add2(sm[j], d);
-        s2[j] = fma2(d, d, s2[j]);
+        sm[j] = add2(sm[j], f[j]);
+        s2[j] = fma2(f[j], f[j], s2[j]);
     }
 }
 // (mean, sum of squared deviations) from the pivot and the sums of differences to it and of their squares
@@ -540,9 +539,9 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksForward) gn_apply_kernel(
     with_activation(a.act, [&](auto act) {
         rows.run([&](Pack<T, V> (&x)[1]) {
             float2 f[P];
-            x[0].unpack(f);
+            x[0].unpack_plus(mean, f);
 #pragma unroll
-            for (int j = 0; j < P; ++j) f[j] = fma2(add2(f[j], mean[j]), scale[j], bias[j]);
+            for (int j = 0; j < P; ++j) f[j] = fma2(f[j], scale[j], bias[j]);
             activate<decltype(act)::value, sizeof(T) == 2, P>(f);
             x[0].pack(f);
             x[0].store(dst);
@@ -605,10 +604,10 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_sums_ke
         with_activation(a.act, [&](auto act) {
             rows.run([&](Pack<T, V> (&x)[2]) {
                 float2 f[P], z[P], g[P];
-                x[0].unpack(f);
+                x[0].unpack_plus(mean, f);
                 x[1].unpack(g);
 #pragma unroll
-                for (int j = 0; j < P; ++j) { f[j] = add2(f[j], mean[j]); z[j] = fma2(f[j], scale[j], bias[j]); }
+                for (int j = 0; j < P; ++j) z[j] = fma2(f[j], scale[j], bias[j]);
                 activate_grad<decltype(act)::value, sizeof(T) == 2, P>(z, g);
 #pragma unroll
                 for (int j = 0; j < P; ++j) { sg[j] = add2(sg[j], g[j]); sgx[j] = fma2(g[j], f[j], sgx[j]); }
@@ -728,10 +727,10 @@ __global__ void __launch_bounds__(kGnThreads, kGnBlocksBackward) gn_grad_input_k
     with_activation(a.act, [&](auto act) {
         rows.run([&](Pack<T, V> (&x)[2]) {
             float2 f[P], z[P], g[P];
-            x[0].unpack(f);
+            x[0].unpack_plus(mean, f);
             x[1].unpack(g);
 #pragma unroll
-            for (int j = 0; j < P; ++j) { f[j] = add2(f[j], mean[j]); z[j] = fma2(f[j], scale[j], bias[j]); }
+            for (int j = 0; j < P; ++j) z[j] = fma2(f[j], scale[j], bias[j]);
             activate_grad<decltype(act)::value, sizeof(T) == 2, P>(z, g);
 #pragma unroll
             for (int j = 0; j < P; ++j) g[j] = fma2(g[j], scale[j], fma2(f[j], m_ux[j], m_u[j]));

@@ -7,8 +7,8 @@
 // the copies.  The share is loaded in four parts and added up part by part as they arrive.
 //
 // What bounds it: the time a block lives, of which the copies take a third and the arithmetic another; about 200 KB
-// per SM are in flight.  32 x 256 x 56^2 bfloat16 with SiLU 32.2 us forward, 60.5 us backward; 64 x 320 x 28^2 25.7 and 45.9 us.
-// (Divisions by powers of two known on the host, and groups looked up in branches, had made those 27.9 and 49.3 us.)
+// per SM are in flight.  32 x 256 x 56^2 bfloat16 with SiLU 31.4 us forward, 58.5 us backward; 64 x 320 x 28^2 25.0 and 44.6 us.
+// (Divisions by powers of two in the kernels, and groups looked up in branches, cost 2.2 and 3.5 us of the latter.)
 // (Clusters that stay and fetch the next sample into a second buffer meanwhile have half the blocks
 // per SM to hide the latency of the sums: 32 x 256 x 56^2 bfloat16 37 us against 34, both before the pivot's one reduction.
 // Clusters that start up to 3 us apart, so that copies and arithmetic of different ones overlap: 3 % faster there, 2 % slower
@@ -171,9 +171,9 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_kernel(const __gri
             for (int i = 0; i < at.count; ++i, dst += at.step) {
                 float2 f[P];
                 Pack<T, V> x = data[i * slots];
-                x.unpack(f);
+                x.unpack_plus(mean, f);
 #pragma unroll
-                for (int j = 0; j < P; ++j) f[j] = fma2(add2(f[j], mean[j]), scale[j], bias[j]);
+                for (int j = 0; j < P; ++j) f[j] = fma2(f[j], scale[j], bias[j]);
                 activate<decltype(act)::value, sizeof(T) == 2, P>(f);
                 x.pack(f);
                 x.store(dst);
@@ -224,10 +224,10 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_grad_kernel(const 
             const int end = min((q + 1) * quarter, at.count);
             for (int i = q * quarter; i < end; ++i) {
                 float2 f[P], z[P], g[P];
-                xs[i * slots].unpack(f);
+                xs[i * slots].unpack_plus(mean, f);
                 ds[i * slots].unpack(g);
 #pragma unroll
-                for (int j = 0; j < P; ++j) { f[j] = add2(f[j], mean[j]); z[j] = fma2(f[j], scale[j], bias[j]); }
+                for (int j = 0; j < P; ++j) z[j] = fma2(f[j], scale[j], bias[j]);
                 activate_grad<decltype(act)::value, sizeof(T) == 2, P>(z, g);
 #pragma unroll
                 for (int j = 0; j < P; ++j) { sg[j] = add2(sg[j], g[j]); sgx[j] = fma2(g[j], f[j], sgx[j]); }
@@ -267,11 +267,11 @@ __global__ void __launch_bounds__(THREADS, PER_SM) gn_cluster_grad_kernel(const 
         with_activation(a.act, [&](auto act) {
             for (int i = 0; i < at.count; ++i, dst += at.step) {
                 float2 f[P], z[P], g[P];
-                xs[i * slots].unpack(f);
+                xs[i * slots].unpack_plus(mean, f);
                 Pack<T, V> d = ds[i * slots];
                 d.unpack(g);
 #pragma unroll
-                for (int j = 0; j < P; ++j) { f[j] = add2(f[j], mean[j]); z[j] = fma2(f[j], scale[j], bias[j]); }
+                for (int j = 0; j < P; ++j) z[j] = fma2(f[j], scale[j], bias[j]);
                 activate_grad<decltype(act)::value, sizeof(T) == 2, P>(z, g);
 #pragma unroll
                 for (int j = 0; j < P; ++j) g[j] = fma2(g[j], scale[j], fma2(f[j], m_ux[j], m_u[j]));
